@@ -70,7 +70,7 @@ const char* fd_last_error(void);
 
 /* Library ABI version (bumped when a signature changes): of this header, and
  * of the library that is loaded. */
-#define FD_ABI_VERSION 14
+#define FD_ABI_VERSION 15
 int fd_abi_version(void);
 
 /* ------------------------------------------------------------------------
@@ -456,6 +456,111 @@ int fd_plan_tiers(
     const int64_t* slot_mapping, int32_t n_tokens,
     int64_t* gpu_slot_mapping, int64_t* host_slot_mapping,
     int32_t* error_count, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Block tables and slot mapping of a step from its requests' lengths.
+ *
+ * What vLLM hands the reference ready-made (block_table, slot_mapping and
+ * seq_lens of fastdecode/backend.py:140-178), made on the GPU. Request
+ * r < n_rows holds context_lens[r] tokens and brings the step's tokens
+ * query_start_loc[r] .. query_start_loc[r + 1] - 1 (q_r of them). With
+ * held_r = ceil(context_lens[r] / block_size) and
+ * need_r = ceil((context_lens[r] + q_r) / block_size) - held_r:
+ *   block_table[r, held_r + k] = free_blocks[taken + sum_{s < r} need_s + k],
+ *                                k < need_r  (in place; other entries stay)
+ *   seq_lens[r]     = context_lens[r] + q_r
+ *   positions[t]    = context_lens[r] + t - query_start_loc[r]   (token t of r)
+ *   slot_mapping[t] = block_table[r, p / block_size] * block_size
+ *                     + p % block_size,  p = positions[t]
+ *   *taken_out      = *taken_in + the blocks taken
+ * free_blocks (num_free ids; the order in which they are to be used, e.g. HBM
+ * blocks before host blocks) may be NULL, with taken_in and taken_out: the
+ * table then holds every block already. taken_in and taken_out are device
+ * int32 and must not be the same: the same call may then be repeated.
+ * Tokens from query_start_loc[n_rows] on (a padded step) get slot -1 and
+ * position 0. A row that needs more than bt_width blocks, that the free list
+ * does not cover any more (rows take in order), of a negative length, or
+ * whose query_start_loc does not lie in order in [0, n_tokens], adds one to
+ * *error_count (may be NULL), takes no block, and its tokens get slot -1; a
+ * token whose block id lies outside [0, num_blocks) adds one and gets slot
+ * -1. Slots of -1 are skipped by fd_reshape_and_cache.
+ * ------------------------------------------------------------------------ */
+int fd_build_tables(
+    const int32_t* query_start_loc, const int32_t* context_lens, int32_t n_rows,
+    int32_t n_tokens, int32_t block_size,
+    int32_t* block_table, int64_t bt_stride, int32_t bt_width, int64_t num_blocks,
+    const int32_t* free_blocks, int32_t num_free, const int32_t* taken_in, int32_t* taken_out,
+    int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens,
+    int32_t* error_count, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of a step's new tokens over the paged cache.
+ *
+ * The prefill form of the GPU tier's attention (flash_attn_varlen_func with a
+ * block table, fastdecode/backend.py:317-327): row i of n brings the query
+ * tokens cu_seqlens_q[i] .. cu_seqlens_q[i + 1] - 1 of q (q_i of them; one is
+ * a decode) and has lens[i] tokens in all, the new ones among them, whose K
+ * and V lie in the cache. For token j of the row and query head h
+ *   out[t, h, :] = softmax(scale * q[t, h] . K_i^T) @ V_i
+ *   lse[h, t]    = logsumexp(scale * q[t, h] . K_i^T)      (natural log)
+ * over the keys 0 .. lens[i] - q_i + j (causal != 0), or all lens[i]
+ * (causal = 0). No key: out = 0, lse = -inf. What lies in keys that a token
+ * does not see (NaN, inf) does not reach it. Cache, table and lens as in
+ * fd_paged_decode_partial; q, out [num_tokens, num_heads, head_size] with
+ * strides (token, head, 1); lse[h * lse_stride_head + t].
+ * A row of more than max_seqlen_q tokens, with lens[i] > bt_width *
+ * block_size, or with a block id outside [0, num_blocks) among its first
+ * ceil(lens[i] / block_size), is a device-side range error: its out and lse
+ * are NaN. A row whose cu_seqlens_q entries do not lie in order in
+ * [0, num_tokens] is not written, nor are tokens outside every row.
+ * workspace: >= fd_prefill_workspace_size(n, num_tokens, ..., max_seqlen_q,
+ * bt_width * block_size, kv_dtype) bytes, as for fd_paged_decode_partial.
+ * Fast kernels: fp16 / bf16 with head_size a multiple of 16 up to 128, or
+ * 256, and fp32 with head_size a multiple of 16 up to 256, where pointers
+ * are 16-byte aligned and strides multiples of 16 bytes; anything else takes
+ * a slower generic kernel.
+ * ------------------------------------------------------------------------ */
+int fd_paged_prefill(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const void* k_cache, const void* v_cache,
+    int64_t kv_stride_block, int64_t kv_stride_head, int64_t kv_stride_token,
+    int64_t num_blocks,
+    const int32_t* block_table, int64_t bt_stride, int32_t bt_width,
+    const int32_t* cu_seqlens_q, const int32_t* lens,
+    int32_t n, int32_t num_tokens, int32_t max_seqlen_q, int32_t causal,
+    int32_t num_heads, int32_t num_kv_heads, int32_t head_size,
+    int32_t block_size, float scale, int32_t kv_dtype,
+    void* out, int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype,
+    float* lse, int64_t lse_stride_head,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over packed keys and values, without a cache (the prefill of fresh
+ * rows over the step's own q/k/v, fastdecode/backend.py:328-340; with causal
+ * = 0 also cross attention to an encoder's states): row i's keys are rows
+ * cu_seqlens_k[i] .. cu_seqlens_k[i + 1] - 1 of k and v [num_keys,
+ * num_kv_heads, head_size], each with strides (token, head, 1). Causal rows
+ * of q_i tokens and L_i keys: token j sees keys 0 .. L_i - q_i + j. A row of
+ * more than max_seqlen_q tokens or max_seqlen_k keys, or whose cu_seqlens_k
+ * entries do not lie in order in [0, num_keys], gives NaN. */
+int fd_varlen_attention(
+    const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+    const void* k, int64_t k_stride_tok, int64_t k_stride_head,
+    const void* v, int64_t v_stride_tok, int64_t v_stride_head,
+    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+    int32_t n, int32_t num_tokens, int32_t num_keys,
+    int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t causal,
+    int32_t num_heads, int32_t num_kv_heads, int32_t head_size,
+    float scale, int32_t dtype,
+    void* out, int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype,
+    float* lse, int64_t lse_stride_head,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Workspace of the two calls above for these sizes (max_keys: bt_width *
+ * block_size, or max_seqlen_k): the partial results of rows whose keys are
+ * divided among workgroups. */
+int fd_prefill_workspace_size(
+    int32_t n, int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_size,
+    int32_t max_seqlen_q, int64_t max_keys, int32_t dtype, size_t* bytes);
 
 /* ------------------------------------------------------------------------
  * Log-sum-exp merge of two partials.

@@ -19,7 +19,7 @@ FD_F16, FD_BF16, FD_F32 = 0, 1, 2
 FD_OK = 0
 FD_ERR_INVALID, FD_ERR_RANGE, FD_ERR_WORKSPACE, FD_ERR_HIP, FD_ERR_UNSUPPORTED = 1, 2, 3, 4, 5
 FD_ERR_RESOURCE = 6
-ABI_VERSION = 14
+ABI_VERSION = 15
 DECODE_COUNTERS = 4096  # FD_DECODE_COUNTERS
 NOALLOC_SCRATCH_BYTES = 32 << 20  # FD_NOALLOC_SCRATCH_BYTES of include/fdattn.h
 
@@ -234,6 +234,56 @@ SIGNATURES: dict[str, tuple] = {
             c_void_p,                              # error_count
             c_void_p,                              # stream
         ],
+    ),
+    "fd_build_tables": (
+        c_int,
+        [
+            c_void_p, c_void_p, c_int32,           # query_start_loc, context_lens, n_rows
+            c_int32, c_int32,                      # n_tokens, block_size
+            c_void_p, c_int64, c_int32, c_int64,   # block_table, stride, width, num_blocks
+            c_void_p, c_int32, c_void_p, c_void_p,  # free_blocks, num_free, taken_in, taken_out
+            c_void_p, c_void_p, c_void_p,          # slot_mapping, positions, seq_lens
+            c_void_p, c_void_p,                    # error_count, stream
+        ],
+    ),
+    "fd_paged_prefill": (
+        c_int,
+        [
+            c_void_p, c_int64, c_int64,            # q, q strides
+            c_void_p, c_void_p,                    # k_cache, v_cache
+            c_int64, c_int64, c_int64,             # kv strides block/head/token
+            c_int64,                               # num_blocks
+            c_void_p, c_int64, c_int32,            # block_table, bt_stride, bt_width
+            c_void_p, c_void_p,                    # cu_seqlens_q, lens
+            c_int32, c_int32, c_int32, c_int32,    # n, num_tokens, max_seqlen_q, causal
+            c_int32, c_int32, c_int32,             # H, KVH, D
+            c_int32, c_float, c_int32,             # block_size, scale, kv_dtype
+            c_void_p, c_int64, c_int64, c_int32,   # out, strides, out_dtype
+            c_void_p, c_int64,                     # lse, lse_stride_head
+            c_void_p, c_size_t, c_void_p,          # workspace, stream
+        ],
+    ),
+    "fd_varlen_attention": (
+        c_int,
+        [
+            c_void_p, c_int64, c_int64,            # q, q strides
+            c_void_p, c_int64, c_int64,            # k, k strides
+            c_void_p, c_int64, c_int64,            # v, v strides
+            c_void_p, c_void_p,                    # cu_seqlens_q, cu_seqlens_k
+            c_int32, c_int32, c_int32,             # n, num_tokens, num_keys
+            c_int32, c_int32, c_int32,             # max_seqlen_q, max_seqlen_k, causal
+            c_int32, c_int32, c_int32,             # H, KVH, D
+            c_float, c_int32,                      # scale, dtype
+            c_void_p, c_int64, c_int64, c_int32,   # out, strides, out_dtype
+            c_void_p, c_int64,                     # lse, lse_stride_head
+            c_void_p, c_size_t, c_void_p,          # workspace, stream
+        ],
+    ),
+    "fd_prefill_workspace_size": (
+        c_int,
+        [c_int32, c_int32, c_int32, c_int32, c_int32,  # n, num_tokens, H, KVH, D
+         c_int32, c_int64, c_int32,                    # max_seqlen_q, max_keys, dtype
+         POINTER(c_size_t)],
     ),
     "fd_merge_attn_states": (
         c_int,

@@ -4,10 +4,10 @@ Mirrors the reference backend's hot path (fastdecode/backend.py) without
 vLLM's base classes:
 
   * `HipOps` / `OPS` -- the seam of backend.py:42-64 (`fa`, `reshape_and_cache`,
-    `merge`, `event`), routed to libfdattn. `fa` implements the paged decode
-    form the split path uses (one query token per row, block table,
-    return_softmax_lse); prefill forms raise NotImplementedError (FlashAttention
-    prefill is not on this path). `split_decode` (no counterpart in the
+    `merge`, `event`), routed to libfdattn. `fa` implements the three forms the
+    reference calls: the S rows' paged decode, the P rows' attention of several
+    tokens over the paged cache, and the F rows' over the step's own q/k/v.
+    `split_decode` (no counterpart in the
     reference) is the fused form of the S rows' two partials and their merge. Tests swap
     OPS the way the reference's tests do (tests/test_plan_and_forward.py:106-113).
   * `build_split_plan` -- FastDecodeMetadataBuilder.build (backend.py:140-178):
@@ -46,22 +46,51 @@ class HipOps:
     @staticmethod
     def fa(q, k, v, cu_seqlens_q=None, max_seqlen_q=1, seqused_k=None, max_seqlen_k=None,
            softmax_scale=None, causal=False, block_table=None, softcap=0.0,
-           return_softmax_lse=False, out=None, row_order=None, total_tokens=None, **_):
-        """Paged decode partial in flash_attn_varlen_func's calling convention
-        (backend.py:306-314): k/v are the [B, BS, KVH, D] cache views, one query
-        token per row, seqused_k the per-row token counts (0 allowed),
-        max_seqlen_k the longest of them (only the table columns it needs are
-        read). Beyond the reference's call: row_order schedules rows (e.g. longest
-        first); total_tokens, the sum of seqused_k known on the host, lets the
-        launch plan size tasks for rows of uneven length."""
-        if block_table is None or max_seqlen_q != 1 or seqused_k is None:
-            raise NotImplementedError("HipOps.fa: only the paged decode form (one query "
-                                      "token per row with a block table) is implemented")
+           return_softmax_lse=False, out=None, row_order=None, total_tokens=None,
+           cu_seqlens_k=None, **other):
+        """Attention in flash_attn_varlen_func's calling convention, in the three
+        forms the reference's backend uses it:
+
+        S (backend.py:306-314): block_table and seqused_k (0 allowed), one query
+        token per row: the paged decode partial. k/v are the [B, BS, KVH, D]
+        cache views, max_seqlen_k the longest row (only the table columns it
+        needs are read). Beyond the reference's call: row_order schedules rows
+        (e.g. longest first); total_tokens, the sum of seqused_k known on the
+        host, lets the launch plan size tasks for rows of uneven length.
+        P (:317-327): block_table and seqused_k, rows of several query tokens
+        (ops.paged_prefill).
+        F (:328-340): cu_seqlens_k, packed k/v [Tk, KVH, D] without a cache
+        (ops.varlen_attention); with causal=False also cross attention."""
+        paged = block_table is not None and seqused_k is not None
+        if not paged and (block_table is not None or cu_seqlens_q is None or cu_seqlens_k is None):
+            raise NotImplementedError("HipOps.fa: a block table with seqused_k, or cu_seqlens_q "
+                                      "with cu_seqlens_k, is needed")
         if softcap:
             raise NotImplementedError("HipOps.fa: logits soft-cap is not supported")
-        o, lse = ops.paged_decode(q, k, v, block_table, seqused_k, softmax_scale, out=out,
-                                  row_order=row_order, max_seqlen_k=max_seqlen_k,
-                                  total_tokens=total_tokens)
+        if paged and max_seqlen_q == 1 and q.shape[0] == block_table.shape[0]:
+            o, lse = ops.paged_decode(q, k, v, block_table, seqused_k, softmax_scale, out=out,
+                                      row_order=row_order, max_seqlen_k=max_seqlen_k,
+                                      total_tokens=total_tokens)
+            return (o, lse) if return_softmax_lse else o
+        window = other.get("window_size")
+        if window is not None and any(w not in (-1, None) for w in window):
+            raise NotImplementedError("HipOps.fa: sliding windows are not supported")
+        for name in ("alibi_slopes", "s_aux", "q_descale", "k_descale", "v_descale"):
+            if other.get(name) is not None:
+                raise NotImplementedError(f"HipOps.fa: {name} is not supported")
+        if paged and cu_seqlens_q is None:
+            raise NotImplementedError("HipOps.fa: rows of several tokens need cu_seqlens_q")
+        if softmax_scale is None:
+            softmax_scale = q.shape[-1] ** -0.5
+        if paged:
+            o, lse = ops.paged_prefill(q, k, v, block_table, cu_seqlens_q, seqused_k,
+                                       softmax_scale, max_seqlen_q, max_seqlen_k=max_seqlen_k,
+                                       causal=causal, out=out)
+        else:
+            if max_seqlen_k is None:
+                max_seqlen_k = k.shape[0]
+            o, lse = ops.varlen_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale,
+                                          max_seqlen_q, max_seqlen_k, causal=causal, out=out)
         return (o, lse) if return_softmax_lse else o
 
     @staticmethod
@@ -95,7 +124,7 @@ OPS = HipOps
 def is_decode_form(kw: dict) -> bool:
     """Whether an OPS.fa call is the split path's paged decode (backend.py:
     306-314: one query token per row over the paged cache, block table and
-    per-row lengths, not causal, no soft-cap), the only form HipOps.fa runs.
+    per-row lengths, not causal, no soft-cap).
     The P rows' causal prefill over the paged cache (:317-327) and the F
     rows' prefill over this step's q/k/v without a block table (:328-340)
     are other forms."""
@@ -104,11 +133,14 @@ def is_decode_form(kw: dict) -> bool:
             and not kw.get("softcap"))
 
 
-def make_ops(prefill_fa):
+def make_ops(prefill_fa=None):
     """The OPS seam for the reference plugin (backend.py:42-64): the paged
     decode form of fa, reshape_and_cache, merge and the fused split go to
     this library; every other form of fa (the P and F prefill calls) goes to
-    `prefill_fa`, i.e. vLLM's flash_attn_varlen_func, unchanged."""
+    `prefill_fa`, e.g. vLLM's flash_attn_varlen_func, unchanged, or where none
+    is given to this library too (HipOps)."""
+    if prefill_fa is None:
+        return HipOps
 
     def fa(**kw):
         if is_decode_form(kw):
@@ -328,9 +360,11 @@ class DeviceStep:
 
 
 def build_device_step(query_start_loc_cpu: torch.Tensor, seq_lens_cpu: torch.Tensor,
-                      block_table: torch.Tensor, slot_mapping: torch.Tensor, num_reqs: int,
+                      block_table: torch.Tensor, slot_mapping: torch.Tensor | None, num_reqs: int,
                       store: state.HostKVStore | None, device) -> DeviceStep | None:
-    """Plans a step on the GPU (fd_plan_tiers): no device-to-host copy. None
+    """Plans a step on the GPU (fd_plan_tiers): no device-to-host copy.
+    slot_mapping None: the step's slots are made there too (ops.build_tables,
+    from the block table and the lengths). None
     when no host tier is set up, or when a prefill row extends prior context
     (whether it touches the host tier is only known on the device; such
     steps take build_split_plan, where the reference's rule applies,
@@ -355,6 +389,10 @@ def build_device_step(query_start_loc_cpu: torch.Tensor, seq_lens_cpu: torch.Ten
     bs = store.block_size
     width = max(1, min(int((int(seq.max()) + bs - 1) // bs), block_table.shape[1]))
     errors = torch.zeros(1, dtype=torch.int32, device=device)
+    if slot_mapping is None:
+        slot_mapping = ops.build_tables(
+            d(qsl.to(torch.int32)), d(ctx.to(torch.int32)), block_table[:num_reqs, :width], bs,
+            n_tok, store.num_gpu_blocks + store.num_cpu_blocks, error_count=errors)[0]
     gpu_bt, cpu_bt, gpu_lens, cpu_lens, gpu_slots, host_slots = ops.plan_tiers(
         block_table[:num_reqs, :width], d(seq.to(torch.int32)), slot_mapping[:n_tok],
         store.num_gpu_blocks, store.num_cpu_blocks, bs, error_count=errors)

@@ -289,6 +289,60 @@ void fill_plan_info(const SplitPlan& sp, int32_t kv_dtype, FdDecodePlan* plan) {
   plan->wave_blocks = sp.fast ? sp.wave_blocks : 0;
 }
 
+// Validates a call over packed query tokens (the keys' side filled in and
+// checked by the caller), completes `a` and launches it.
+int run_prefill(PrefillArgs& a, const char* who, const void* q, int64_t q_stride_tok,
+                int64_t q_stride_head, const int32_t* cu_seqlens_q, int32_t n,
+                int32_t num_tokens, int32_t max_seqlen_q, int32_t causal, int32_t num_heads,
+                int32_t num_kv_heads, int32_t head_size, float scale, int32_t dtype, void* out,
+                int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype, float* lse,
+                int64_t lse_stride_head, void* workspace, size_t workspace_bytes, void* stream) {
+  if (n < 0 || num_tokens < 0 || max_seqlen_q < 0)
+    return set_error(FD_ERR_INVALID, "%s: negative size", who);
+  if (num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0)
+    return set_error(FD_ERR_INVALID,
+                     "%s: num_heads must be a multiple of num_kv_heads (%d, %d)", who, num_heads,
+                     num_kv_heads);
+  if (head_size <= 0 || head_size > 512)
+    return set_error(FD_ERR_UNSUPPORTED, "%s: head_size %d outside 1..512", who, head_size);
+  if (!valid_dtype(dtype)) return set_error(FD_ERR_INVALID, "%s: unsupported dtype %d", who, dtype);
+  if (out_dtype != dtype && out_dtype != FD_F32)
+    return set_error(FD_ERR_INVALID, "%s: out dtype must equal the kv dtype or be fp32", who);
+  if (!std::isfinite(scale)) return set_error(FD_ERR_INVALID, "%s: scale is not finite", who);
+  if (n == 0 || num_tokens == 0) return FD_OK;
+  if (!q || !out || !lse || !cu_seqlens_q)
+    return set_error(FD_ERR_INVALID, "%s: NULL tensor pointer", who);
+  if ((!a.k || !a.v) && (a.bt != nullptr ? a.num_blocks > 0 : a.Tk > 0))
+    return set_error(FD_ERR_INVALID, "%s: NULL tensor pointer", who);
+  a.q = q;
+  a.q_st = q_stride_tok;
+  a.q_sh = q_stride_head;
+  a.cu_q = cu_seqlens_q;
+  a.n = n;
+  a.T = num_tokens;
+  a.H = num_heads;
+  a.KVH = num_kv_heads;
+  a.D = head_size;
+  a.max_q = max_seqlen_q;
+  a.causal = causal != 0;
+  a.scale = scale;
+  a.dt = dtype;
+  a.out = out;
+  a.out_st = out_stride_tok;
+  a.out_sh = out_stride_head;
+  a.out_dt = out_dtype;
+  a.lse = lse;
+  a.lse_sh = lse_stride_head;
+  a.workspace = workspace;
+  const size_t need = prefill_workspace_bytes(n, num_tokens, num_heads, num_kv_heads, head_size,
+                                              max_seqlen_q, a.max_k, dtype);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(FD_ERR_WORKSPACE,
+                     "%s: workspace of %zu bytes (16-byte aligned) required, got %zu", who, need,
+                     workspace == nullptr ? (size_t)0 : workspace_bytes);
+  return launch_prefill(a, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
 }  // namespace
 }  // namespace fd
 
@@ -574,6 +628,118 @@ int fd_plan_tiers(const int32_t* block_table, int64_t bt_stride, int32_t bt_widt
   a.host_slots = host_slot_mapping;
   a.error_count = error_count;
   return launch_plan_tiers(a, static_cast<hipStream_t>(stream));
+}
+
+int fd_build_tables(const int32_t* query_start_loc, const int32_t* context_lens, int32_t n_rows,
+                    int32_t n_tokens, int32_t block_size, int32_t* block_table, int64_t bt_stride,
+                    int32_t bt_width, int64_t num_blocks, const int32_t* free_blocks,
+                    int32_t num_free, const int32_t* taken_in, int32_t* taken_out,
+                    int64_t* slot_mapping, int64_t* positions, int32_t* seq_lens,
+                    int32_t* error_count, void* stream) {
+  if (n_rows < 0 || n_tokens < 0 || bt_width < 0 || num_blocks < 0 || num_free < 0)
+    return set_error(FD_ERR_INVALID, "build_tables: negative size");
+  if (block_size <= 0) return set_error(FD_ERR_INVALID, "build_tables: block_size must be > 0");
+  if (bt_stride < bt_width)
+    return set_error(FD_ERR_INVALID, "build_tables: bt_stride %lld < bt_width %d",
+                     (long long)bt_stride, bt_width);
+  if (n_rows > 0 && (!query_start_loc || !context_lens || !seq_lens ||
+                     (bt_width > 0 && !block_table)))
+    return set_error(FD_ERR_INVALID, "build_tables: NULL tensor pointer");
+  if (n_tokens > 0 && (!slot_mapping || !positions))
+    return set_error(FD_ERR_INVALID, "build_tables: NULL slot_mapping or positions");
+  if ((free_blocks != nullptr || num_free > 0 || taken_in != nullptr || taken_out != nullptr) &&
+      (!free_blocks || !taken_in || !taken_out))
+    return set_error(FD_ERR_INVALID,
+                     "build_tables: free_blocks, taken_in and taken_out go together");
+  if (free_blocks != nullptr && taken_in == taken_out)
+    return set_error(FD_ERR_INVALID, "build_tables: taken_in and taken_out must differ");
+  const BuildTablesArgs a{query_start_loc, context_lens, n_rows,    n_tokens,  block_size,
+                          block_table,     bt_stride,    bt_width,  num_blocks, free_blocks,
+                          num_free,        taken_in,     taken_out, slot_mapping, positions,
+                          seq_lens,        error_count};
+  return launch_build_tables(a, static_cast<hipStream_t>(stream));
+}
+
+int fd_paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
+                     const void* k_cache, const void* v_cache, int64_t kv_stride_block,
+                     int64_t kv_stride_head, int64_t kv_stride_token, int64_t num_blocks,
+                     const int32_t* block_table, int64_t bt_stride, int32_t bt_width,
+                     const int32_t* cu_seqlens_q, const int32_t* lens, int32_t n,
+                     int32_t num_tokens, int32_t max_seqlen_q, int32_t causal, int32_t num_heads,
+                     int32_t num_kv_heads, int32_t head_size, int32_t block_size, float scale,
+                     int32_t kv_dtype, void* out, int64_t out_stride_tok, int64_t out_stride_head,
+                     int32_t out_dtype, float* lse, int64_t lse_stride_head, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  if (block_size <= 0)
+    return set_error(FD_ERR_INVALID, "paged_prefill: block_size must be > 0");
+  if (bt_width < 0 || num_blocks < 0)
+    return set_error(FD_ERR_INVALID, "paged_prefill: negative size");
+  if (bt_width > 0 && bt_stride < bt_width)
+    return set_error(FD_ERR_INVALID, "paged_prefill: bt_stride %lld < bt_width %d",
+                     (long long)bt_stride, bt_width);
+  if (n > 0 && num_tokens > 0 && (!block_table || !lens))
+    return set_error(FD_ERR_INVALID, "paged_prefill: NULL tensor pointer");
+  PrefillArgs a{};
+  a.k = k_cache;
+  a.v = v_cache;
+  a.k_sb = a.v_sb = kv_stride_block;
+  a.k_sh = a.v_sh = kv_stride_head;
+  a.k_st = a.v_st = kv_stride_token;
+  a.num_blocks = num_blocks;
+  a.bt = block_table;
+  a.bt_stride = bt_stride;
+  a.bt_width = bt_width;
+  a.BS = block_size;
+  a.lens = lens;
+  a.max_k = (int32_t)std::min<int64_t>((int64_t)bt_width * block_size, INT32_MAX);
+  return run_prefill(a, "paged_prefill", q, q_stride_tok, q_stride_head, cu_seqlens_q, n,
+                     num_tokens, max_seqlen_q, causal, num_heads, num_kv_heads, head_size, scale,
+                     kv_dtype, out, out_stride_tok, out_stride_head, out_dtype, lse,
+                     lse_stride_head, workspace, workspace_bytes, stream);
+}
+
+int fd_varlen_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k,
+                        int64_t k_stride_tok, int64_t k_stride_head, const void* v,
+                        int64_t v_stride_tok, int64_t v_stride_head, const int32_t* cu_seqlens_q,
+                        const int32_t* cu_seqlens_k, int32_t n, int32_t num_tokens,
+                        int32_t num_keys, int32_t max_seqlen_q, int32_t max_seqlen_k,
+                        int32_t causal, int32_t num_heads, int32_t num_kv_heads,
+                        int32_t head_size, float scale, int32_t dtype, void* out,
+                        int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype,
+                        float* lse, int64_t lse_stride_head, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  if (num_keys < 0 || max_seqlen_k < 0)
+    return set_error(FD_ERR_INVALID, "varlen_attention: negative size");
+  if (n > 0 && num_tokens > 0 && !cu_seqlens_k)
+    return set_error(FD_ERR_INVALID, "varlen_attention: NULL tensor pointer");
+  PrefillArgs a{};
+  a.k = k;
+  a.v = v;
+  a.k_sh = k_stride_head;
+  a.k_st = k_stride_tok;
+  a.v_sh = v_stride_head;
+  a.v_st = v_stride_tok;
+  a.BS = 1;
+  a.cu_k = cu_seqlens_k;
+  a.Tk = num_keys;
+  a.max_k = max_seqlen_k;
+  return run_prefill(a, "varlen_attention", q, q_stride_tok, q_stride_head, cu_seqlens_q, n,
+                     num_tokens, max_seqlen_q, causal, num_heads, num_kv_heads, head_size, scale,
+                     dtype, out, out_stride_tok, out_stride_head, out_dtype, lse,
+                     lse_stride_head, workspace, workspace_bytes, stream);
+}
+
+int fd_prefill_workspace_size(int32_t n, int32_t num_tokens, int32_t num_heads,
+                              int32_t num_kv_heads, int32_t head_size, int32_t max_seqlen_q,
+                              int64_t max_keys, int32_t dtype, size_t* bytes) {
+  if (bytes == nullptr) return set_error(FD_ERR_INVALID, "prefill_workspace_size: bytes is NULL");
+  if (n < 0 || num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads != 0 || head_size <= 0 || max_seqlen_q < 0 || max_keys < 0 ||
+      !valid_dtype(dtype))
+    return set_error(FD_ERR_INVALID, "prefill_workspace_size: bad sizes");
+  *bytes = prefill_workspace_bytes(n, num_tokens, num_heads, num_kv_heads, head_size,
+                                   max_seqlen_q, max_keys, dtype);
+  return FD_OK;
 }
 
 int fd_merge_attn_states(void* out, int64_t out_stride_seq, int64_t out_stride_head,

@@ -378,4 +378,56 @@ struct PlanTiersArgs {
 };
 int launch_plan_tiers(const PlanTiersArgs& a, hipStream_t s);
 
+// Attention of packed query tokens (prefill.h): rows of several new tokens
+// over a paged cache (bt != NULL) or over packed keys and values.
+struct PrefillArgs {
+  const void* q;
+  int64_t q_st, q_sh;  // element strides: token, head
+  const void* k;
+  const void* v;
+  int64_t k_sb, k_sh, k_st;  // block (paged only), head, token
+  int64_t v_sb, v_sh, v_st;
+  int64_t num_blocks;  // paged
+  const int32_t* bt;
+  int64_t bt_stride;
+  int32_t bt_width, BS;
+  const int32_t* cu_q;  // [n + 1]
+  const int32_t* lens;  // paged: [n] tokens in all
+  const int32_t* cu_k;  // packed: [n + 1]
+  int32_t n, T, Tk;     // rows, query tokens, packed keys
+  int32_t H, KVH, D, max_q, max_k, causal;
+  float scale;
+  int32_t dt, out_dt;
+  void* out;
+  int64_t out_st, out_sh;
+  float* lse;
+  int64_t lse_sh;
+  void* workspace;
+};
+int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s);
+// Workspace that a call of these sizes needs (kv_tokens: the longest row's
+// keys as far as the host knows).
+size_t prefill_workspace_bytes(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_t D,
+                               int32_t max_q, int64_t max_k, int32_t dt);
+
+// Block tables, slot mapping, positions and lengths of a step (build_tables.hip).
+struct BuildTablesArgs {
+  const int32_t* qsl;  // [n + 1]
+  const int32_t* ctx;  // [n]
+  int32_t n, T, BS;
+  int32_t* bt;
+  int64_t bt_stride;
+  int32_t bt_width;
+  int64_t num_blocks;
+  const int32_t* free_blocks;  // may be NULL: no blocks are taken
+  int32_t num_free;
+  const int32_t* taken_in;
+  int32_t* taken_out;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* seq_lens;
+  int32_t* error_count;
+};
+int launch_build_tables(const BuildTablesArgs& a, hipStream_t s);
+
 }  // namespace fd

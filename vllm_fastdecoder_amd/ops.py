@@ -962,6 +962,256 @@ def plan_tiers(block_table: torch.Tensor, seq_lens: torch.Tensor, slot_mapping: 
     return gpu_bt, cpu_bt, gpu_lens, cpu_lens, gpu_slots, host_slots
 
 
+def _one_device(dev: torch.device, **tensors: torch.Tensor) -> None:
+    """Every GPU tensor of a call lies on the device it launches on (pinned
+    host tensors are reached from any)."""
+    for name, t in tensors.items():
+        _require(not t.is_cuda or t.device == dev, f"{name} must be on {dev}, not {t.device}")
+
+
+def _launch(dev: torch.device, fn, *args) -> None:
+    """A library call on `dev`, which need not be the current device."""
+    if dev.index is not None and dev.index != _current_device():
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args))
+    else:
+        _lib.check(fn(*args))
+
+
+_PREFILL_WS_SIZES: dict = {}
+
+
+def prefill_workspace_bytes(n: int, num_tokens: int, H: int, KVH: int, D: int, max_seqlen_q: int,
+                            max_keys: int, dtype: torch.dtype) -> int:
+    """Workspace a paged_prefill (max_keys: its table's columns times the block
+    size) or varlen_attention (max_keys: max_seqlen_k) call of these sizes
+    needs on the current device (fd_prefill_workspace_size, remembered). For
+    reserve_workspace ahead of a graph capture."""
+    key = (n, num_tokens, H, KVH, D, max_seqlen_q, max_keys, dtype, _current_device())
+    size = _PREFILL_WS_SIZES.get(key)
+    if size is None:
+        c = ctypes.c_size_t()
+        _lib.check(_lib.load_lib().fd_prefill_workspace_size(n, num_tokens, H, KVH, D,
+                                                             max_seqlen_q, max_keys, _DT[dtype],
+                                                             ctypes.byref(c)))
+        size = int(c.value)
+        if len(_PREFILL_WS_SIZES) > 4096:
+            _PREFILL_WS_SIZES.clear()
+        _PREFILL_WS_SIZES[key] = size
+    return size
+
+
+def _prefill_args(q, k, v, cu_seqlens_q, max_seqlen_q, out, lse):
+    """The checks paged_prefill and varlen_attention share; out and lse made
+    where the caller brings none."""
+    _require(q.is_cuda and q.dim() == 3, "q must be [T, H, D] on the GPU")
+    T, H, D = q.shape
+    _require(k.dim() == v.dim() and k.shape == v.shape, "k and v must be of one shape")
+    _require(k.shape[-1] == D, "head size mismatch")
+    KVH = k.shape[-2]
+    _require(KVH > 0 and H % KVH == 0, "num_heads must be a multiple of num_kv_heads")
+    _dtype_code(q, "q")
+    _require(k.dtype == q.dtype and v.dtype == q.dtype, "q, k and v must share a dtype")
+    if out is None:
+        out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty(H, T, dtype=torch.float32, device=q.device)
+    _require(out.is_cuda and out.shape == q.shape, "out must be [T, H, D] on the GPU")
+    _require(out.dtype == q.dtype or out.dtype == torch.float32, "out must be q's dtype or float32")
+    _require(lse.is_cuda and lse.dtype == torch.float32 and tuple(lse.shape) == (H, T)
+             and (T <= 1 or lse.stride(1) == 1), "lse must be float32 [H, T] with contiguous rows")
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        _require(D == 1 or t.stride(-1) == 1, f"{name} must be contiguous in head_size")
+    _require(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.dim() == 1
+             and cu_seqlens_q.shape[0] >= 1, "cu_seqlens_q must be int32 [n + 1]")
+    _require(max_seqlen_q >= 0, "max_seqlen_q must be >= 0")
+    _one_device(q.device, k=k, v=v, out=out, lse=lse, cu_seqlens_q=cu_seqlens_q)
+    return T, H, D, KVH, cu_seqlens_q.shape[0] - 1, out, lse
+
+
+def paged_prefill(
+    q: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    seqused_k: torch.Tensor,
+    softmax_scale: float,
+    max_seqlen_q: int,
+    max_seqlen_k: int | None = None,
+    causal: bool = True,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of rows that bring several new tokens each (a prompt's chunk,
+    tokens to verify; one token is a decode) over the paged cache, where their
+    K and V already lie: the P rows' call of flash_attn_varlen_func at
+    fastdecode/backend.py:317-327 (fd_paged_prefill).
+
+    q [T, H, D]: row i's tokens are cu_seqlens_q[i] .. cu_seqlens_q[i + 1] - 1
+    (int32 [n + 1]); key_cache / value_cache [B, BS, KVH, D] views; block_table
+    int32 [n, W]; seqused_k int32 [n] tokens of each row in all. Token j of a
+    row of q_i sees keys 0 .. seqused_k[i] - q_i + j (causal), or all of them.
+    max_seqlen_q (the most tokens a row brings) and max_seqlen_k (the longest
+    row: only the columns it needs are planned for; None: the table's width)
+    are ints the host knows; a longer row is a range error, as is a block id
+    outside the cache: its out and lse are NaN. Returns out [T, H, D] (q's
+    dtype unless given) and lse [H, T] float32; a token without keys gives 0
+    and -inf, tokens in no row are not written."""
+    _require(key_cache.dim() == 4 and value_cache.shape == key_cache.shape
+             and key_cache.stride() == value_cache.stride(),
+             "key_cache/value_cache must be [B, BS, KVH, D] of one shape and strides")
+    T, H, D, KVH, n, out, lse = _prefill_args(q, key_cache, value_cache, cu_seqlens_q,
+                                              max_seqlen_q, out, lse)
+    B, BS = key_cache.shape[:2]
+    _require(block_table.dtype == torch.int32 and seqused_k.dtype == torch.int32,
+             "block_table and seqused_k must be int32")
+    _require(block_table.dim() == 2 and block_table.shape[0] == n and seqused_k.shape == (n,),
+             "block_table must be [n, W] and seqused_k [n]")
+    dev = q.device
+    _one_device(dev, block_table=block_table, seqused_k=seqused_k)
+    if n == 0 or T == 0:
+        return out, lse
+    if max_seqlen_k is not None:
+        cols = max(1, -(-int(max_seqlen_k) // BS))
+        if cols < block_table.shape[1]:
+            block_table = block_table[:, :cols]
+    W = block_table.shape[1]
+    bt, bt_ptr = _table_on_device(block_table, dev)
+    _require(W <= 1 or bt.stride(1) == 1, "block_table rows must be contiguous")
+    ln = _on_device(seqused_k, dev).contiguous()
+    cu = _on_device(cu_seqlens_q, dev).contiguous()
+    ws = WORKSPACE.get(dev, prefill_workspace_bytes(n, T, H, KVH, D, int(max_seqlen_q), W * BS,
+                                                    q.dtype))
+    _launch(dev, _lib.load_lib().fd_paged_prefill,
+            q.data_ptr(), q.stride(0), q.stride(1), device_ptr(key_cache), device_ptr(value_cache),
+            key_cache.stride(0), key_cache.stride(2), key_cache.stride(1), B,
+            bt_ptr, max(bt.stride(0), W) if n == 1 else bt.stride(0), W, cu.data_ptr(),
+            ln.data_ptr(), n, T, int(max_seqlen_q), int(bool(causal)), H, KVH, D, BS,
+            float(softmax_scale), _DT[q.dtype], out.data_ptr(), out.stride(0), out.stride(1),
+            _DT[out.dtype], lse.data_ptr(), lse.stride(0),
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            _stream_for(q))
+    return out, lse
+
+
+def varlen_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor,
+    softmax_scale: float,
+    max_seqlen_q: int,
+    max_seqlen_k: int,
+    causal: bool = False,
+    out: torch.Tensor | None = None,
+    lse: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention over packed keys and values, without a cache: the F rows' call
+    of flash_attn_varlen_func at fastdecode/backend.py:328-340 (causal, k and v
+    the step's own), and cross attention to an encoder's states of another
+    length (not causal) (fd_varlen_attention).
+
+    q [T, H, D], k / v [Tk, KVH, D] (strided views of a fused projection are
+    fine); row i's tokens are cu_seqlens_q[i] .. cu_seqlens_q[i + 1] - 1, its
+    keys likewise (int32 [n + 1] each). Causal: token j of q_i sees keys
+    0 .. k_i - q_i + j. max_seqlen_q / max_seqlen_k as for paged_prefill.
+    Returns out [T, H, D] and lse [H, T] float32; a token without keys gives 0
+    and -inf, tokens in no row are not written."""
+    _require(k.dim() == 3, "k and v must be [Tk, KVH, D]")
+    T, H, D, KVH, n, out, lse = _prefill_args(q, k, v, cu_seqlens_q, max_seqlen_q, out, lse)
+    _require(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.shape == (n + 1,),
+             "cu_seqlens_k must be int32 [n + 1]")
+    _require(max_seqlen_k >= 0, "max_seqlen_k must be >= 0")
+    dev = q.device
+    _one_device(dev, cu_seqlens_k=cu_seqlens_k)
+    if n == 0 or T == 0:
+        return out, lse
+    cu = _on_device(cu_seqlens_q, dev).contiguous()
+    cuk = _on_device(cu_seqlens_k, dev).contiguous()
+    ws = WORKSPACE.get(dev, prefill_workspace_bytes(n, T, H, KVH, D, int(max_seqlen_q),
+                                                    int(max_seqlen_k), q.dtype))
+    _launch(dev, _lib.load_lib().fd_varlen_attention,
+            q.data_ptr(), q.stride(0), q.stride(1), device_ptr(k), k.stride(0), k.stride(1),
+            device_ptr(v), v.stride(0), v.stride(1), cu.data_ptr(), cuk.data_ptr(), n, T,
+            k.shape[0], int(max_seqlen_q), int(max_seqlen_k), int(bool(causal)), H, KVH, D,
+            float(softmax_scale), _DT[q.dtype], out.data_ptr(), out.stride(0), out.stride(1),
+            _DT[out.dtype], lse.data_ptr(), lse.stride(0),
+            ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+            _stream_for(q))
+    return out, lse
+
+
+def build_tables(
+    query_start_loc: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    block_size: int,
+    num_tokens: int,
+    num_blocks: int,
+    free_blocks: torch.Tensor | None = None,
+    taken: torch.Tensor | None = None,
+    error_count: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """A step's new cache blocks, slot mapping, positions and lengths from its
+    requests' lengths, on the GPU (fd_build_tables): the inputs of plan_tiers,
+    reshape_and_cache and paged_prefill, which the reference takes from vLLM
+    (fastdecode/backend.py:140-178).
+
+    query_start_loc int32 [n + 1], context_lens int32 [n] (tokens each request
+    already holds), block_table int32 [n, W]; num_tokens: slots to make (at
+    least query_start_loc[n]; those past it are -1); num_blocks: ids the
+    step's caches hold, both tiers together. With free_blocks (int32 [F], in
+    the order of use) and taken (int32 [1], how many are used up) the blocks
+    that the new tokens need are written into block_table behind each row's
+    held ones; without them the table holds every block already. Returns
+    (slot_mapping int64 [num_tokens], positions int64 [num_tokens], seq_lens
+    int32 [n], the new count of taken blocks or None). error_count: int32 [1]
+    GPU counter of rows and tokens that got no slot (see include/fdattn.h)."""
+    _require(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2,
+             "block_table must be int32 [n, W] on the GPU")
+    n, W = block_table.shape
+    dev = block_table.device
+    _require(n == 0 or W <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous")
+    _require(n <= 1 or block_table.stride(0) >= W, "block_table rows must not overlap")
+    _require(query_start_loc.dtype == torch.int32 and query_start_loc.shape == (n + 1,),
+             "query_start_loc must be int32 [n + 1]")
+    _require(context_lens.dtype == torch.int32 and context_lens.shape == (n,),
+             "context_lens must be int32 [n]")
+    _require(block_size > 0, "block_size must be > 0")
+    _require(num_tokens >= 0 and num_blocks >= 0, "num_tokens and num_blocks must be >= 0")
+    _require((free_blocks is None) == (taken is None), "free_blocks and taken go together")
+    _one_device(dev, query_start_loc=query_start_loc, context_lens=context_lens)
+    qsl = _on_device(query_start_loc, dev).contiguous()
+    ctx = _on_device(context_lens, dev).contiguous()
+    taken_out = None
+    if free_blocks is not None:
+        _require(free_blocks.is_cuda and free_blocks.dtype == torch.int32
+                 and free_blocks.dim() == 1 and free_blocks.is_contiguous(),
+                 "free_blocks must be a contiguous int32 GPU tensor")
+        _require(taken.is_cuda and taken.dtype == torch.int32 and taken.shape == (1,),
+                 "taken must be int32 [1] on the GPU")
+        _one_device(dev, free_blocks=free_blocks, taken=taken)
+        taken_out = torch.empty_like(taken)
+    if error_count is not None:
+        _one_device(dev, error_count=error_count)
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    seq_lens = torch.empty(n, dtype=torch.int32, device=dev)
+    num_free = free_blocks.numel() if free_blocks is not None else 0
+    _launch(dev, _lib.load_lib().fd_build_tables,
+            qsl.data_ptr(), ctx.data_ptr(), n, int(num_tokens), int(block_size),
+            block_table.data_ptr(), block_table.stride(0) if n > 1 else W, W, int(num_blocks),
+            # (a list of no blocks still needs an address)
+            None if free_blocks is None else free_blocks.data_ptr() or taken.data_ptr(), num_free,
+            taken.data_ptr() if taken is not None else None,
+            taken_out.data_ptr() if taken_out is not None else None,
+            slots.data_ptr(), positions.data_ptr(), seq_lens.data_ptr(),
+            _device_counter(error_count, "error_count"), _stream_for(block_table))
+    return slots, positions, seq_lens, taken_out
+
+
 def longest_first(lens: torch.Tensor) -> torch.Tensor:
     """int32 permutation of the rows by decreasing length, computed on the
     host (the planner already holds the lengths there)."""
