@@ -60,6 +60,67 @@ __device__ __forceinline__ int last_row(int n, int64_t x, F&& f) {
   return lo;
 }
 
+// One query token and head over keys [from, to) of its row, one key after
+// another with a running maximum and sum, by a wave: lane l holds elements
+// l + 64 k of the head. acc is the sum of weights exp(s - m) times V.
+template <int kPerLane>
+__device__ __forceinline__ void scalar_attention(const PrefillArgs& a, int i, const PrefillRow& r,
+                                                 int t, int h, int from, int to, float& m, float& l,
+                                                 float (&acc)[kPerLane]) {
+  const int lane = threadIdx.x % kWave;
+  const int kh = h / (a.H / a.KVH);
+  const bool paged = a.bt != nullptr;
+  float qv[kPerLane];
+  const int64_t qbase = (int64_t)t * a.q_st + (int64_t)h * a.q_sh;
+#pragma unroll
+  for (int x = 0; x < kPerLane; ++x) {
+    const int d = lane + x * kWave;
+    qv[x] = d < a.D ? load_elem(a.q, qbase + d, a.dt) : 0.f;
+    acc[x] = 0.f;
+  }
+  m = neg_inf();
+  l = 0.f;
+  for (int key = from; key < to; ++key) {
+    const int64_t id = paged ? a.bt[(int64_t)i * a.bt_stride + key / a.BS] : r.k0 + key;
+    const int64_t in = paged ? key % a.BS : 0;
+    const int64_t kb = id * (paged ? a.k_sb : a.k_st) + in * a.k_st + (int64_t)kh * a.k_sh;
+    const int64_t vb = id * (paged ? a.v_sb : a.v_st) + in * a.v_st + (int64_t)kh * a.v_sh;
+    float s = 0.f;
+#pragma unroll
+    for (int x = 0; x < kPerLane; ++x) {
+      const int d = lane + x * kWave;
+      if (d < a.D) s += qv[x] * load_elem(a.k, kb + d, a.dt);
+    }
+    s = wave_sum(s) * a.scale;
+    const float mn = fmaxf(m, s);
+    const float base = mn == neg_inf() ? 0.f : mn;  // every score so far -inf
+    const float alpha = __expf(m - base);
+    const float p = __expf(s - base);
+    l = l * alpha + p;
+#pragma unroll
+    for (int x = 0; x < kPerLane; ++x) {
+      const int d = lane + x * kWave;
+      if (d < a.D) acc[x] = acc[x] * alpha + p * load_elem(a.v, vb + d, a.dt);
+    }
+    m = mn;
+  }
+}
+
+// Its result as out and lse.
+template <int kPerLane>
+__device__ __forceinline__ void scalar_store(const PrefillArgs& a, int t, int h, float m, float l,
+                                             const float (&acc)[kPerLane]) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t obase = (int64_t)t * a.out_st + (int64_t)h * a.out_sh;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int x = 0; x < kPerLane; ++x) {
+    const int d = lane + x * kWave;
+    if (d < a.D) store_elem(a.out, obase + d, a.out_dt, acc[x] * inv);
+  }
+  if (lane == 0) a.lse[(int64_t)h * a.lse_sh + t] = l == 0.f ? neg_inf() : m + __logf(l);
+}
+
 int launch_prefill_generic(const PrefillArgs& a, hipStream_t s);
 
 }  // namespace fd
