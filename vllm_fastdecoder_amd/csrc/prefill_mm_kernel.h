@@ -56,6 +56,7 @@ typedef s16x4 __attribute__((address_space(3))) * lds_s16x4_ptr;
 constexpr int kPfWaves = 4;
 constexpr int kPfThreads = kPfWaves * kWave;
 constexpr float kLazyRescale = 8.f;  // log2 units
+constexpr int kReadAhead = 4;        // operands read ahead of their product
 
 template <typename T>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -120,6 +121,24 @@ struct PfShape {
   static constexpr int kLds = kStages > kMergeBytes ? kStages : kMergeBytes;
 };
 
+// kCount products, each behind the LDS reads of the product kAhead further on:
+// read(x) gives product x's operand, use(x, operand) computes it. In this
+// order by force: left to itself the compiler reads each operand right ahead
+// of its product, which then waits for it.
+template <int kCount, int kAhead, typename R, typename U>
+__device__ __forceinline__ void read_ahead(R&& read, U&& use) {
+  u32x4 buf[kAhead];
+#pragma unroll
+  for (int x = 0; x < kAhead && x < kCount; ++x) buf[x] = read(x);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int x = 0; x < kCount; ++x) {
+    use(x, buf[x % kAhead]);
+    if (x + kAhead < kCount) buf[x % kAhead] = read(x + kAhead);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // The first lane's value, known to be every lane's.
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -183,44 +202,45 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
   const char* vbase = static_cast<const char*>(a.v) + (int64_t)kvh * a.v_sh * 2;
   const bool paged = a.bt != nullptr;
   const int32_t* bt = paged ? a.bt + (int64_t)i * a.bt_stride : nullptr;
-  // block (paged) or packed row of the wave's loads of a step, and the key
-  // itself (past the row's end: its last)
+  // Where a step's keys lie: lane k of every wave looks key k up (past the
+  // row's end: its last), the block id a step ahead; the loads, 16 bytes of a
+  // row a lane, take their row's offset from that lane.
   bool bad = false;
-  int idx[NJ];
-  auto key_of = [&](int step, int j) {
-    const int u = (j * kPfWaves + wave) * kWave + lane;
-    return min(step * KTB + u / CPR, r.nk - 1);
-  };
-  auto fetch_ids = [&](int step) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int key = key_of(step, j);
-      if (paged)
-        idx[j] = bt[(uint32_t)(((uint64_t)(uint32_t)key * p.bs_magic) >> p.bs_shift)];
-      else
-        idx[j] = r.k0 + key;
-    }
+  const bool one_offset = a.k_sb == a.v_sb && a.k_st == a.v_st;
+  auto key_of = [&](int step) { return min(step * KTB + lane % KTB, r.nk - 1); };
+  auto block_of = [&](int key) { return (int)(((uint64_t)(uint32_t)key * p.bs_magic) >> p.bs_shift); };
+  int next_id = 0;
+  auto fetch_id = [&](int step) {
+    const int key = key_of(step);
+    next_id = paged ? bt[block_of(key)] : r.k0 + key;
   };
   auto issue = [&](int step, int stage) {
+    int id = next_id, in = 0;
+    if (paged) {
+      const bool ok = (uint32_t)id < (uint64_t)a.num_blocks;
+      bad |= !ok;
+      id = ok ? id : 0;
+      const int key = key_of(step);
+      in = key - block_of(key) * a.BS;
+    }
+    const int64_t ko = ((int64_t)id * a.k_sb + (int64_t)in * a.k_st) * 2;
+    const int64_t vo = one_offset ? ko : ((int64_t)id * a.v_sb + (int64_t)in * a.v_st) * 2;
+    auto of_lane = [](int64_t x, int src) {
+      const uint32_t lo = __builtin_amdgcn_ds_bpermute(src * 4, (int)(uint32_t)x);
+      const uint32_t hi = __builtin_amdgcn_ds_bpermute(src * 4, (int)(uint32_t)((uint64_t)x >> 32));
+      return (int64_t)((uint64_t)hi << 32 | lo);
+    };
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       if (LOADS % kPfWaves != 0 && j * kPfWaves + wave >= LOADS) break;
       const int u = (j * kPfWaves + wave) * kWave + lane;
       const int row = u / CPR, c = u - row * CPR;
-      int id = idx[j], in = 0;
-      if (paged) {
-        const bool ok = (uint32_t)id < (uint64_t)a.num_blocks;
-        bad |= !ok;
-        id = ok ? id : 0;
-        const int key = key_of(step, j);
-        in = key - (int)(((uint64_t)(uint32_t)key * p.bs_magic) >> p.bs_shift) * a.BS;
-      }
-      const int64_t ko = (int64_t)id * a.k_sb + (int64_t)in * a.k_st;
-      const int64_t vo = (int64_t)id * a.v_sb + (int64_t)in * a.v_st;
+      const int64_t kj = of_lane(ko, row);
+      const int64_t vj = one_offset ? kj : of_lane(vo, row);
       const uint32_t at = lds0 + stage * 2 * PfShape<D>::kStageBytes +
                           (j * kPfWaves + wave) * (kWave * 16);
-      load_lds16(kbase + ko * 2 + 16 * (c ^ Swizzle<D>::k(row)), at);
-      load_lds16(vbase + vo * 2 + 16 * (c ^ Swizzle<D>::v(row)), at + PfShape<D>::kStageBytes);
+      load_lds16(kbase + 16 * (c ^ Swizzle<D>::k(row)) + kj, at);
+      load_lds16(vbase + 16 * (c ^ Swizzle<D>::v(row)) + vj, at + PfShape<D>::kStageBytes);
     }
   };
 
@@ -242,9 +262,9 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
       for (int e = 0; e < 16; ++e) acc[db][e] = 0.f;
 
     if (s_from < s_to) {
-      fetch_ids(s_from);
+      fetch_id(s_from);
       issue(s_from, 0);
-      if (s_from + 1 < s_to) fetch_ids(s_from + 1);
+      if (s_from + 1 < s_to) fetch_id(s_from + 1);
     }
     for (int step = s_from; step < s_to; ++step) {
       const int stage = (step - s_from) & 1;
@@ -252,7 +272,7 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
       __syncthreads();
       if (step + 1 < s_to) {
         issue(step + 1, stage ^ 1);
-        if (step + 2 < s_to) fetch_ids(step + 2);
+        if (step + 2 < s_to) fetch_id(step + 2);
       }
       const int key0 = step * KTB + wk * KT;
       if (!works || key0 > vis_hi) continue;
@@ -261,18 +281,16 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
 
       f32x16 s[NB];
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int row = krow + 32 * nb;
-        const char* kr = ks_lds + row * PfShape<D>::kRowBytes;
-        const int sw = Swizzle<D>::k(row);
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[nb][e] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(kr + 16 * ((2 * ks + half) ^ sw));
-          s[nb] = mfma32<T>(kf, q[ks], s[nb]);
-        }
-      }
+      read_ahead<KS * NB, kReadAhead>(
+          [&](int x) {
+            const int row = krow + 32 * (x % NB), c = 2 * (x / NB) + half;
+            return *reinterpret_cast<const u32x4*>(ks_lds + row * PfShape<D>::kRowBytes +
+                                                   16 * (c ^ Swizzle<D>::k(row)));
+          },
+          [&](int x, const u32x4& kf) { s[x % NB] = mfma32<T>(kf, q[x / NB], s[x % NB]); });
       const bool masked = key0 + KT - 1 > vis_lo;
       if (masked) {
 #pragma unroll
@@ -326,10 +344,9 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
         const uint2 xu = __builtin_bit_cast(uint2, x), yu = __builtin_bit_cast(uint2, y);
         return u32x4{xu.x, xu.y, yu.x, yu.y};
       };
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int kk = 0; kk < 2 * NB; ++kk) acc[db] = mfma32<T>(v_frag(kk, db), pf[kk], acc[db]);
+      read_ahead<DB * 2 * NB, kReadAhead>(
+          [&](int x) { return v_frag(x / DB, x % DB); },
+          [&](int x, const u32x4& vf) { acc[x % DB] = mfma32<T>(vf, pf[x / DB], acc[x % DB]); });
     }
 
     // anything that is not finite came from the inputs, or from values that a
@@ -486,7 +503,8 @@ __device__ __forceinline__ void pf_fill_nan(const PrefillMmParams& p, const Pref
 // heads fastest, so that an XCD keeps to few of them and a kv head's keys stay
 // in its L2.
 template <typename T, int D>
-__global__ __launch_bounds__(kPfThreads, 2) void prefill_mm_kernel(PrefillMmParams p) {
+__global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+prefill_mm_kernel(PrefillMmParams p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ PfShared sh;
   const PrefillArgs& a = p.a;
