@@ -159,15 +159,18 @@ PrefillPlan plan_prefill_mm(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_
 
 size_t prefill_workspace_bytes(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_t D,
                                int32_t max_q, int64_t max_k, int32_t dt) {
-  if (dt == FD_F32 || !mm_head_size(D)) return 0;
+  if (!mm_head_size(D)) return 0;
   return plan_prefill_mm(n, T, H, KVH, D, max_q, max_k).workspace;
 }
 
 int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s) {
   (void)workspace_bytes;
   auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-  auto strides = [](int64_t x, int64_t y) { return x >= 0 && y >= 0 && x % 8 == 0 && y % 8 == 0; };
-  const bool fast = a.dt != FD_F32 && mm_head_size(a.D) && aligned(a.q) && aligned(a.k) &&
+  const int unit = a.dt == FD_F32 ? 4 : 8;  // elements of 16 bytes
+  auto strides = [&](int64_t x, int64_t y) {
+    return x >= 0 && y >= 0 && x % unit == 0 && y % unit == 0;
+  };
+  const bool fast = mm_head_size(a.D) && aligned(a.q) && aligned(a.k) &&
                     aligned(a.v) && aligned(a.out) && strides(a.q_st, a.q_sh) &&
                     strides(a.out_st, a.out_sh) && strides(a.k_st, a.k_sh) &&
                     strides(a.v_st, a.v_sh) && strides(a.k_sb, a.v_sb) &&
@@ -184,7 +187,7 @@ int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s) 
   // (a scale of 0 makes all scores alike, which a scale too small to show does
   // too; its product with -inf, a masked score, is still -inf)
   const float scale = a.scale * kLog2e;
-  p.q_flip = scale < 0.f ? 0x80008000u : 0u;
+  p.q_flip = scale >= 0.f ? 0u : a.dt == FD_F32 ? 0x80000000u : 0x80008000u;
   p.scale_log2 = scale == 0.f ? 0x1p-100f : std::fabs(scale);
   int sh = 0;
   while ((1ll << sh) < a.BS) ++sh;
@@ -198,7 +201,9 @@ int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s) 
   const int64_t tasks =
       ((int64_t)p.plan.tiles_a * p.plan.sa + (int64_t)p.plan.rows_b * p.plan.sb) * a.KVH;
   if (tasks > INT32_MAX) return set_error(FD_ERR_UNSUPPORTED, "prefill: too many tasks");
-  const int rc = a.dt == FD_F16 ? launch_prefill_mm_f16(p, s) : launch_prefill_mm_bf16(p, s);
+  const int rc = a.dt == FD_F16    ? launch_prefill_mm_f16(p, s)
+                 : a.dt == FD_BF16 ? launch_prefill_mm_bf16(p, s)
+                                   : launch_prefill_mm_f32(p, s);
   if (rc != FD_OK || (p.plan.sa <= 1 && p.plan.sb <= 1)) return rc;
   return launch_prefill_combine(p, s);
 }

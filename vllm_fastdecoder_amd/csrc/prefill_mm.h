@@ -1,4 +1,4 @@
-// Attention of packed query tokens on the matrix cores (fp16 / bf16): the
+// Attention of packed query tokens on the matrix cores: the
 // kernel's plan and launcher, shared by prefill.hip (planning) and the
 // translation units that instantiate it per type.
 #pragma once
@@ -25,7 +25,7 @@ struct PrefillMmParams {
   PrefillPlan plan;
   int32_t G;
   float scale_log2;      // > 0
-  uint32_t q_flip;       // sign bits to flip in q (a negative scale)
+  uint32_t q_flip;       // sign bits to flip in a word of q (a negative scale)
   uint32_t bs_magic;     // key / BS = key * bs_magic >> bs_shift, key < 2^31
   int32_t bs_shift;
   float* part_o;   // [parts][T * H][D]
@@ -36,6 +36,7 @@ PrefillPlan plan_prefill_mm(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_
                             int64_t max_k);
 int launch_prefill_mm_f16(const PrefillMmParams& p, hipStream_t s);
 int launch_prefill_mm_bf16(const PrefillMmParams& p, hipStream_t s);
+int launch_prefill_mm_f32(const PrefillMmParams& p, hipStream_t s);
 int launch_prefill_combine(const PrefillMmParams& p, hipStream_t s);
 
 }  // namespace fd

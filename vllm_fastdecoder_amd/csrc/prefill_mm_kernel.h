@@ -1,5 +1,6 @@
 // Attention of packed query tokens with both products on the matrix cores,
-// instantiated per type by prefill_mm_f16.hip and prefill_mm_bf16.hip.
+// instantiated per type by prefill_mm_f16.hip, prefill_mm_bf16.hip and
+// prefill_mm_f32.hip.
 //
 // A workgroup of four waves takes a tile of query rows of one kv head and
 // walks the tile's keys. Query rows are (token, head of the kv head's group)
@@ -21,6 +22,9 @@
 //                   8 + 4 h .. + 3 of each 16, and V^T's A operand is read in
 //                   that order (two ds_read_b64_tr_b16, whose lane mapping is
 //                   told in decode_mm.hip), so no lane ever moves a weight.
+// fp32 goes the same way with v_mfma_f32_32x32x2: a chunk of 16 bytes is an
+// operand of four products (whose two dims are 4 apart, in K and Q alike), and
+// the weights are P^T's operand without a conversion.
 // P is rounded to the inputs' type (fp16: scaled by 2^7, so that small weights
 // stay normal), its sum is taken in fp32 before the rounding; the error it
 // adds is of the size of the output's own rounding.
@@ -60,6 +64,7 @@ constexpr int kReadAhead = 4;        // operands read ahead of their product
 
 template <typename T>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  static_assert(!std::is_same<T, F32>::value, "16-bit types");
   if constexpr (std::is_same<T, F16>::value)
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a),
                                                   __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
@@ -99,25 +104,30 @@ __device__ __forceinline__ void load_lds16(const char* g, uint32_t lds) {
       : "memory");
 }
 
-// Rows of D 16-bit elements in LDS: kPeriod rows start at different multiples
-// of the 256 bytes that all banks serve at once.
-template <int D>
+// Rows of kBytes in LDS: kPeriod rows start at different multiples of the 256
+// bytes that all banks serve at once. (fp32 V rows are read 32 floats in a
+// row at a time and need none.)
+template <int kBytes, bool kF32>
 struct Swizzle {
-  static constexpr int kPeriod = D % 128 == 0 ? 1 : D % 64 == 0 ? 2 : D % 32 == 0 ? 4 : 8;
+  static constexpr int kPeriod = kBytes % 256 == 0 ? 1 : kBytes % 128 == 0 ? 2 : kBytes % 64 == 0 ? 4 : 8;
   static __device__ __forceinline__ int k(int row) { return (row / kPeriod) & (16 / kPeriod - 1); }
   static __device__ __forceinline__ int v(int row) {
-    return kPeriod < 4 ? ((row / kPeriod) & (4 / kPeriod - 1)) << 2 : 0;
+    return !kF32 && kPeriod < 4 ? ((row / kPeriod) & (4 / kPeriod - 1)) << 2 : 0;
   }
 };
 
-template <int D>
+template <typename T, int D>
 struct PfShape {
-  static constexpr int kStepKeys = D <= 128 ? 64 : 32;       // keys of a step
-  static constexpr int kRowBytes = D * 2;
+  static constexpr bool kF32 = std::is_same<T, F32>::value;
+  static constexpr int kElt = kF32 ? 4 : 2;
+  static constexpr int kStepKeys = kElt * D <= 256 ? 64 : 32;  // keys of a step
+  static constexpr int kRowBytes = D * kElt;
+  // waves a SIMD holds by the registers that a wave needs
+  static constexpr int kWavesPerSimd = kF32 && D > 128 ? 1 : 2;
   static constexpr int kStageBytes = kStepKeys * kRowBytes;  // of K, and of V
   // the merge of a B tile's two key waves: fp32 accumulators of half the waves
   static constexpr int kMergeBytes = 2 * ((D + 31) / 32 * 32) * 32 * 4;
-  static constexpr int kStages = 4 * kStageBytes + 64;  // (reads past D in the last row)
+  static constexpr int kStages = 4 * kStageBytes + 32 * kElt;  // (reads past D in the last row)
   static constexpr int kLds = kStages > kMergeBytes ? kStages : kMergeBytes;
 };
 
@@ -154,13 +164,16 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
                                         int row0, int kvh, int part, int parts, char* lds,
                                         PfShared& sh, int tid) {
   static_assert(WQ * WK == kPfWaves, "four waves");
-  constexpr int KTB = PfShape<D>::kStepKeys;
+  constexpr bool F = PfShape<T, D>::kF32;
+  constexpr int ES = PfShape<T, D>::kElt;
+  constexpr int KTB = PfShape<T, D>::kStepKeys;
+  using Swz = Swizzle<PfShape<T, D>::kRowBytes, F>;
   constexpr int KT = KTB / WK;
   static_assert(KT % 32 == 0, "32 keys a wave at least");
   constexpr int NB = KT / 32;         // key blocks of a wave's step
-  constexpr int KS = D / 16;          // steps over the dims of a score
+  constexpr int KS = F ? D / 8 : D / 16;  // 16-byte operands over the dims of a score
   constexpr int DB = (D + 31) / 32;   // blocks of output dims
-  constexpr int CPR = D / 8;          // 16-byte chunks of a row
+  constexpr int CPR = D * ES / 16;    // 16-byte chunks of a row
   constexpr int LOADS = KTB * CPR / kWave;                       // per step, of K and of V
   constexpr int NJ = (LOADS + kPfWaves - 1) / kPfWaves;          // per wave
   constexpr float kShift = std::is_same<T, F16>::value ? 7.f : 0.f;
@@ -185,21 +198,21 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
   const int per = (steps + parts - 1) / parts;
   const int s_from = uniform(min(steps, part * per)), s_to = uniform(min(steps, s_from + per));
 
-  // Q: row col's dims 16 ks + 8 half .. + 7
+  // Q: row col's chunks 2 ks + half of 16 bytes
   u32x4 q[KS];
   {
-    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (int64_t)(r.q0 + tok) * a.q_st +
-                         (int64_t)head * a.q_sh + 8 * half;
+    const char* qp = static_cast<const char*>(a.q) +
+                     ((int64_t)(r.q0 + tok) * a.q_st + (int64_t)head * a.q_sh) * ES + 16 * half;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-      q[ks] = *reinterpret_cast<const u32x4*>(qp + 16 * ks);
+      q[ks] = *reinterpret_cast<const u32x4*>(qp + 32 * ks);
       q[ks] ^= p.q_flip;
     }
   }
 
   const uint32_t lds0 = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds);
-  const char* kbase = static_cast<const char*>(a.k) + (int64_t)kvh * a.k_sh * 2;
-  const char* vbase = static_cast<const char*>(a.v) + (int64_t)kvh * a.v_sh * 2;
+  const char* kbase = static_cast<const char*>(a.k) + (int64_t)kvh * a.k_sh * ES;
+  const char* vbase = static_cast<const char*>(a.v) + (int64_t)kvh * a.v_sh * ES;
   const bool paged = a.bt != nullptr;
   const int32_t* bt = paged ? a.bt + (int64_t)i * a.bt_stride : nullptr;
   // Where a step's keys lie: lane k of every wave looks key k up (past the
@@ -223,8 +236,8 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
       const int key = key_of(step);
       in = key - block_of(key) * a.BS;
     }
-    const int64_t ko = ((int64_t)id * a.k_sb + (int64_t)in * a.k_st) * 2;
-    const int64_t vo = one_offset ? ko : ((int64_t)id * a.v_sb + (int64_t)in * a.v_st) * 2;
+    const int64_t ko = ((int64_t)id * a.k_sb + (int64_t)in * a.k_st) * ES;
+    const int64_t vo = one_offset ? ko : ((int64_t)id * a.v_sb + (int64_t)in * a.v_st) * ES;
     auto of_lane = [](int64_t x, int src) {
       const uint32_t lo = __builtin_amdgcn_ds_bpermute(src * 4, (int)(uint32_t)x);
       const uint32_t hi = __builtin_amdgcn_ds_bpermute(src * 4, (int)(uint32_t)((uint64_t)x >> 32));
@@ -237,10 +250,10 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
       const int row = u / CPR, c = u - row * CPR;
       const int64_t kj = of_lane(ko, row);
       const int64_t vj = one_offset ? kj : of_lane(vo, row);
-      const uint32_t at = lds0 + stage * 2 * PfShape<D>::kStageBytes +
+      const uint32_t at = lds0 + stage * 2 * PfShape<T, D>::kStageBytes +
                           (j * kPfWaves + wave) * (kWave * 16);
-      load_lds16(kbase + 16 * (c ^ Swizzle<D>::k(row)) + kj, at);
-      load_lds16(vbase + 16 * (c ^ Swizzle<D>::v(row)) + vj, at + PfShape<D>::kStageBytes);
+      load_lds16(kbase + 16 * (c ^ Swz::k(row)) + kj, at);
+      load_lds16(vbase + 16 * (c ^ Swz::v(row)) + vj, at + PfShape<T, D>::kStageBytes);
     }
   };
 
@@ -276,8 +289,8 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
       }
       const int key0 = step * KTB + wk * KT;
       if (!works || key0 > vis_hi) continue;
-      const char* ks_lds = lds + stage * 2 * PfShape<D>::kStageBytes;
-      const char* vs_lds = ks_lds + PfShape<D>::kStageBytes;
+      const char* ks_lds = lds + stage * 2 * PfShape<T, D>::kStageBytes;
+      const char* vs_lds = ks_lds + PfShape<T, D>::kStageBytes;
 
       f32x16 s[NB];
 #pragma unroll
@@ -287,10 +300,19 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
       read_ahead<KS * NB, kReadAhead>(
           [&](int x) {
             const int row = krow + 32 * (x % NB), c = 2 * (x / NB) + half;
-            return *reinterpret_cast<const u32x4*>(ks_lds + row * PfShape<D>::kRowBytes +
-                                                   16 * (c ^ Swizzle<D>::k(row)));
+            return *reinterpret_cast<const u32x4*>(ks_lds + row * PfShape<T, D>::kRowBytes +
+                                                   16 * (c ^ Swz::k(row)));
           },
-          [&](int x, const u32x4& kf) { s[x % NB] = mfma32<T>(kf, q[x / NB], s[x % NB]); });
+          [&](int x, const u32x4& kf) {
+            if constexpr (F) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[x % NB] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                    __uint_as_float(kf[e]), __uint_as_float(q[x / NB][e]), s[x % NB], 0, 0, 0);
+            } else {
+              s[x % NB] = mfma32<T>(kf, q[x / NB], s[x % NB]);
+            }
+          });
       const bool masked = key0 + KT - 1 > vis_lo;
       if (masked) {
 #pragma unroll
@@ -319,34 +341,66 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
           for (int e = 0; e < 16; ++e) acc[db][e] *= alpha;
       }
       const float ms = (m == neg_inf() ? 0.f : m) - kShift;
-      u32x4 pf[2 * NB];
       float sum = 0.f;
+      if constexpr (F) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float pv[16];
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          pv[e] = fast_exp2(fmaf(s[nb][e], p.scale_log2, -ms));
-          sum += pv[e];
+          for (int e = 0; e < 16; ++e) {
+            s[nb][e] = fast_exp2(fmaf(s[nb][e], p.scale_log2, -ms));
+            sum += s[nb][e];
+          }
+        l += sum;
+        // operand x: keys 8 g + 4 half .. + 3 of block nb, one dim a lane
+        read_ahead<DB * 4 * NB, 2>(
+            [&](int x) {
+              const int db = x % DB, g = x / DB;  // (g counts over the blocks)
+              const char* pv = vs_lds + (wk * KT + 8 * g + 4 * half) * PfShape<T, D>::kRowBytes +
+                               (32 * db + col) * 4;
+              u32x4 v;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v[e] = *reinterpret_cast<const uint32_t*>(pv + e * PfShape<T, D>::kRowBytes);
+              return v;
+            },
+            [&](int x, const u32x4& v) {
+              const int db = x % DB, g = x / DB;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                    __uint_as_float(v[e]), s[g / 4][4 * (g % 4) + e], acc[db], 0, 0, 0);
+            });
+      } else {
+        u32x4 pf[2 * NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float pv[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            pv[e] = fast_exp2(fmaf(s[nb][e], p.scale_log2, -ms));
+            sum += pv[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 2)
+            pf[2 * nb + e / 8][(e % 8) / 2] = pack2<T>(pv[e], pv[e + 1]);
         }
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) pf[2 * nb + e / 8][(e % 8) / 2] = pack2<T>(pv[e], pv[e + 1]);
+        l += sum;
+        read_ahead<DB * 2 * NB, kReadAhead>(
+            [&](int x) {
+              const int r0 = vrow + 16 * (x / DB);  // and 8 rows on
+              const int d = 32 * (x % DB) + vdim;
+              const char* p0 = vs_lds + r0 * PfShape<T, D>::kRowBytes +
+                               (((d >> 3) ^ Swz::v(r0)) << 4) + (d & 7) * 2;
+              const char* p1 = vs_lds + (r0 + 8) * PfShape<T, D>::kRowBytes +
+                               (((d >> 3) ^ Swz::v(r0 + 8)) << 4) + (d & 7) * 2;
+              const uint2 v0 = __builtin_bit_cast(
+                  uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p0));
+              const uint2 v1 = __builtin_bit_cast(
+                  uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p1));
+              return u32x4{v0.x, v0.y, v1.x, v1.y};
+            },
+            [&](int x, const u32x4& vf) { acc[x % DB] = mfma32<T>(vf, pf[x / DB], acc[x % DB]); });
       }
-      l += sum;
-      auto v_frag = [&](int kk, int db) -> u32x4 {
-        const int r0 = vrow + 16 * kk;  // and 8 rows on
-        const int d = 32 * db + vdim;
-        const char* p0 = vs_lds + r0 * PfShape<D>::kRowBytes + (((d >> 3) ^ Swizzle<D>::v(r0)) << 4) + (d & 7) * 2;
-        const char* p1 = vs_lds + (r0 + 8) * PfShape<D>::kRowBytes +
-                         (((d >> 3) ^ Swizzle<D>::v(r0 + 8)) << 4) + (d & 7) * 2;
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p0);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)p1);
-        const uint2 xu = __builtin_bit_cast(uint2, x), yu = __builtin_bit_cast(uint2, y);
-        return u32x4{xu.x, xu.y, yu.x, yu.y};
-      };
-      read_ahead<DB * 2 * NB, kReadAhead>(
-          [&](int x) { return v_frag(x / DB, x % DB); },
-          [&](int x, const u32x4& vf) { acc[x % DB] = mfma32<T>(vf, pf[x / DB], acc[x % DB]); });
     }
 
     // anything that is not finite came from the inputs, or from values that a
@@ -429,9 +483,9 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, int i, const P
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = l == 0.f && !bad ? 0.f : acc[db][4 * g + e] * inv;
       const int64_t o = ob + 32 * db + 8 * g;
-      if (a.out_dt == FD_F32) {
+      if (F || a.out_dt == FD_F32) {
         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + o) = make_float4(y[0], y[1], y[2], y[3]);
-      } else {
+      } else if constexpr (!F) {
         uint2 u;
         u.x = to_out(T{}, y[0]) | ((uint32_t)to_out(T{}, y[1]) << 16);
         u.y = to_out(T{}, y[2]) | ((uint32_t)to_out(T{}, y[3]) << 16);
@@ -503,7 +557,7 @@ __device__ __forceinline__ void pf_fill_nan(const PrefillMmParams& p, const Pref
 // heads fastest, so that an XCD keeps to few of them and a kv head's keys stay
 // in its L2.
 template <typename T, int D>
-__global__ __launch_bounds__(kPfThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+__global__ __launch_bounds__(kPfThreads, (PfShape<T, D>::kWavesPerSimd)) void
 prefill_mm_kernel(PrefillMmParams p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ PfShared sh;
@@ -581,23 +635,24 @@ prefill_mm_kernel(PrefillMmParams p) {
     pf_fill_nan(p, r, row0, is_a ? kRowsA : kRowsB, kvh, part, parts);
     return;
   }
-  constexpr int kWk = PfShape<D>::kStepKeys / 32;  // key waves of a B tile
+  constexpr int kWk = PfShape<T, D>::kStepKeys / 32;  // key waves of a B tile
   const int tid = threadIdx.x;
   const bool done = is_a
                         ? pf_tile<T, D, 4, 1>(p, i, r, row0, kvh, part, parts, lds, sh, tid)
                         : pf_tile<T, D, 4 / kWk, kWk>(p, i, r, row0, kvh, part, parts, lds, sh, tid);
   if (!done)
-    pf_tile_scalar<D, PfShape<D>::kStepKeys>(p, i, r, row0, is_a ? kRowsA : kRowsB, kvh, part, parts);
+    pf_tile_scalar<D, PfShape<T, D>::kStepKeys>(p, i, r, row0, is_a ? kRowsA : kRowsB, kvh, part, parts);
 }
 
 template <typename T, int D>
 hipError_t launch_d(const PrefillMmParams& p, hipStream_t s) {
   const int64_t tasks = ((int64_t)p.plan.tiles_a * p.plan.sa + (int64_t)p.plan.rows_b * p.plan.sb) * p.a.KVH;
   const auto kernel = prefill_mm_kernel<T, D>;
+  constexpr int kLds = PfShape<T, D>::kLds;
   static const hipError_t set = hipFuncSetAttribute(
-      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, PfShape<D>::kLds);
+      reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   if (set != hipSuccess) return set;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tasks), dim3(kPfThreads), PfShape<D>::kLds, s, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)tasks), dim3(kPfThreads), kLds, s, p);
   return hipGetLastError();
 }
 
