@@ -514,7 +514,11 @@ int fd_build_tables(
  * are NaN. A row whose cu_seqlens_q entries do not lie in order in
  * [0, num_tokens] is not written, nor are tokens outside every row.
  * workspace: >= fd_prefill_workspace_size(n, num_tokens, ..., max_seqlen_q,
- * bt_width * block_size, kv_dtype) bytes, as for fd_paged_decode_partial.
+ * bt_width * block_size, block_size, kv_dtype) bytes, as for fd_paged_decode_partial;
+ * counters: NULL, or the caller's arrival counters as for
+ * fd_paged_decode_counted (the same array may serve both, in stream order),
+ * which save a call whose rows are divided among workgroups the launch that
+ * clears counters in the workspace.
  * Fast kernels: fp16 / bf16 with head_size a multiple of 16 up to 128, or
  * 256, and fp32 with head_size a multiple of 16 up to 256, where pointers
  * are 16-byte aligned and strides multiples of 16 bytes; anything else takes
@@ -532,7 +536,7 @@ int fd_paged_prefill(
     int32_t block_size, float scale, int32_t kv_dtype,
     void* out, int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype,
     float* lse, int64_t lse_stride_head,
-    void* workspace, size_t workspace_bytes, void* stream);
+    void* workspace, size_t workspace_bytes, void* stream, uint32_t* counters);
 
 /* The same over packed keys and values, without a cache (the prefill of fresh
  * rows over the step's own q/k/v, fastdecode/backend.py:328-340; with causal
@@ -553,14 +557,14 @@ int fd_varlen_attention(
     float scale, int32_t dtype,
     void* out, int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype,
     float* lse, int64_t lse_stride_head,
-    void* workspace, size_t workspace_bytes, void* stream);
+    void* workspace, size_t workspace_bytes, void* stream, uint32_t* counters);
 
-/* Workspace of the two calls above for these sizes (max_keys: bt_width *
- * block_size, or max_seqlen_k): the partial results of rows whose keys are
- * divided among workgroups. */
+/* Workspace of the two calls above for these sizes (paged: max_keys =
+ * bt_width * block_size; packed: max_seqlen_k, with block_size 0): the partial
+ * results of rows whose keys are divided among workgroups. */
 int fd_prefill_workspace_size(
     int32_t n, int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_size,
-    int32_t max_seqlen_q, int64_t max_keys, int32_t dtype, size_t* bytes);
+    int32_t max_seqlen_q, int64_t max_keys, int32_t block_size, int32_t dtype, size_t* bytes);
 
 /* ------------------------------------------------------------------------
  * Log-sum-exp merge of two partials.

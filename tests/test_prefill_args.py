@@ -15,7 +15,8 @@ P = 4096  # a pointer that is never followed
 def _paged(**over):
     a = dict(q=P, qst=512, qsh=64, k=P, v=P, sb=4096, sh=128, st=256, B=9, bt=P, bts=8, W=8, cu=P,
              lens=P, n=2, T=7, mq=5, causal=1, H=8, KVH=2, D=64, BS=16, scale=0.1, dt=0, out=P,
-             ost=512, osh=64, odt=0, lse=P, lsh=7, ws=None, wsb=0, stream=None)
+             ost=512, osh=64, odt=0, lse=P, lsh=7, ws=None, wsb=0, stream=None,
+             counters=None)
     a.update(over)
     return _lib.load_lib().fd_paged_prefill(*a.values())
 
@@ -23,7 +24,7 @@ def _paged(**over):
 def _varlen(**over):
     a = dict(q=P, qst=512, qsh=64, k=P, kst=128, ksh=64, v=P, vst=128, vsh=64, cuq=P, cuk=P, n=2,
              T=7, Tk=30, mq=5, mk=20, causal=0, H=8, KVH=2, D=64, scale=0.1, dt=0, out=P, ost=512,
-             osh=64, odt=0, lse=P, lsh=7, ws=None, wsb=0, stream=None)
+             osh=64, odt=0, lse=P, lsh=7, ws=None, wsb=0, stream=None, counters=None)
     a.update(over)
     return _lib.load_lib().fd_varlen_attention(*a.values())
 
@@ -70,13 +71,13 @@ def test_calls_of_no_tokens_launch_nothing():
 
 
 @pytest.mark.parametrize("over", [dict(n=-1), dict(T=-1), dict(H=0), dict(KVH=3), dict(D=0),
-                                  dict(mq=-1), dict(mk=-1), dict(dt=5)], ids=str)
+                                  dict(mq=-1), dict(mk=-1), dict(BS=-1), dict(dt=5)], ids=str)
 def test_workspace_size_refuses(over):
-    a = dict(n=2, T=7, H=8, KVH=2, D=64, mq=5, mk=20, dt=0)
+    a = dict(n=2, T=7, H=8, KVH=2, D=64, mq=5, mk=20, BS=16, dt=0)
     size = ctypes.c_size_t()
     assert _lib.load_lib().fd_prefill_workspace_size(*a.values(), ctypes.byref(size)) == 0
     a.update(over)
     assert _lib.load_lib().fd_prefill_workspace_size(*a.values(), ctypes.byref(size)) \
         == _lib.FD_ERR_INVALID
-    a = dict(n=2, T=7, H=8, KVH=2, D=64, mq=5, mk=20, dt=0)
+    a = dict(n=2, T=7, H=8, KVH=2, D=64, mq=5, mk=20, BS=16, dt=0)
     assert _lib.load_lib().fd_prefill_workspace_size(*a.values(), None) == _lib.FD_ERR_INVALID

@@ -261,6 +261,7 @@ SIGNATURES: dict[str, tuple] = {
             c_void_p, c_int64, c_int64, c_int32,   # out, strides, out_dtype
             c_void_p, c_int64,                     # lse, lse_stride_head
             c_void_p, c_size_t, c_void_p,          # workspace, stream
+            c_void_p,                              # counters
         ],
     ),
     "fd_varlen_attention": (
@@ -277,12 +278,13 @@ SIGNATURES: dict[str, tuple] = {
             c_void_p, c_int64, c_int64, c_int32,   # out, strides, out_dtype
             c_void_p, c_int64,                     # lse, lse_stride_head
             c_void_p, c_size_t, c_void_p,          # workspace, stream
+            c_void_p,                              # counters
         ],
     ),
     "fd_prefill_workspace_size": (
         c_int,
         [c_int32, c_int32, c_int32, c_int32, c_int32,  # n, num_tokens, H, KVH, D
-         c_int32, c_int64, c_int32,                    # max_seqlen_q, max_keys, dtype
+         c_int32, c_int64, c_int32, c_int32,           # max_seqlen_q, max_keys, block_size, dtype
          POINTER(c_size_t)],
     ),
     "fd_merge_attn_states": (

@@ -37,9 +37,13 @@ HIPCC_FLAGS = [
 # default heuristic its P.V accumulators live in AGPRs, and the rarely taken
 # rescale branch of every block makes the compiler copy all 32 of them to
 # VGPRs and back on the common path too (64 v_accvgpr moves per block); in
-# VGPRs the kernel needs 154 registers and no AGPRs.
+# VGPRs the kernel needs 154 registers and no AGPRs. prefill_mm_*.hip: the
+# same, for the rescale of their accumulators.
 SOURCE_FLAGS = {
     "decode_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "prefill_mm_f16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "prefill_mm_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "prefill_mm_f32.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 CXX_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-pthread", "-Wall", "-Wno-unused-function"]

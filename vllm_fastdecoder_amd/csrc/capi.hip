@@ -335,12 +335,13 @@ int run_prefill(PrefillArgs& a, const char* who, const void* q, int64_t q_stride
   a.lse_sh = lse_stride_head;
   a.workspace = workspace;
   const size_t need = prefill_workspace_bytes(n, num_tokens, num_heads, num_kv_heads, head_size,
-                                              max_seqlen_q, a.max_k, dtype);
+                                              max_seqlen_q, a.max_k, a.bt != nullptr ? a.BS : 0,
+                                              dtype);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
     return set_error(FD_ERR_WORKSPACE,
                      "%s: workspace of %zu bytes (16-byte aligned) required, got %zu", who, need,
                      workspace == nullptr ? (size_t)0 : workspace_bytes);
-  return launch_prefill(a, workspace_bytes, static_cast<hipStream_t>(stream));
+  return launch_prefill(a, static_cast<hipStream_t>(stream));
 }
 
 }  // namespace
@@ -669,7 +670,7 @@ int fd_paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                      int32_t num_kv_heads, int32_t head_size, int32_t block_size, float scale,
                      int32_t kv_dtype, void* out, int64_t out_stride_tok, int64_t out_stride_head,
                      int32_t out_dtype, float* lse, int64_t lse_stride_head, void* workspace,
-                     size_t workspace_bytes, void* stream) {
+                     size_t workspace_bytes, void* stream, uint32_t* counters) {
   if (block_size <= 0)
     return set_error(FD_ERR_INVALID, "paged_prefill: block_size must be > 0");
   if (bt_width < 0 || num_blocks < 0)
@@ -680,6 +681,7 @@ int fd_paged_prefill(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   if (n > 0 && num_tokens > 0 && (!block_table || !lens))
     return set_error(FD_ERR_INVALID, "paged_prefill: NULL tensor pointer");
   PrefillArgs a{};
+  a.counters = counter_array(counters);
   a.k = k_cache;
   a.v = v_cache;
   a.k_sb = a.v_sb = kv_stride_block;
@@ -707,12 +709,13 @@ int fd_varlen_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_he
                         int32_t head_size, float scale, int32_t dtype, void* out,
                         int64_t out_stride_tok, int64_t out_stride_head, int32_t out_dtype,
                         float* lse, int64_t lse_stride_head, void* workspace,
-                        size_t workspace_bytes, void* stream) {
+                        size_t workspace_bytes, void* stream, uint32_t* counters) {
   if (num_keys < 0 || max_seqlen_k < 0)
     return set_error(FD_ERR_INVALID, "varlen_attention: negative size");
   if (n > 0 && num_tokens > 0 && !cu_seqlens_k)
     return set_error(FD_ERR_INVALID, "varlen_attention: NULL tensor pointer");
   PrefillArgs a{};
+  a.counters = counter_array(counters);
   a.k = k;
   a.v = v;
   a.k_sh = k_stride_head;
@@ -731,14 +734,15 @@ int fd_varlen_attention(const void* q, int64_t q_stride_tok, int64_t q_stride_he
 
 int fd_prefill_workspace_size(int32_t n, int32_t num_tokens, int32_t num_heads,
                               int32_t num_kv_heads, int32_t head_size, int32_t max_seqlen_q,
-                              int64_t max_keys, int32_t dtype, size_t* bytes) {
+                              int64_t max_keys, int32_t block_size, int32_t dtype,
+                              size_t* bytes) {
   if (bytes == nullptr) return set_error(FD_ERR_INVALID, "prefill_workspace_size: bytes is NULL");
   if (n < 0 || num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 ||
       num_heads % num_kv_heads != 0 || head_size <= 0 || max_seqlen_q < 0 || max_keys < 0 ||
-      !valid_dtype(dtype))
+      block_size < 0 || !valid_dtype(dtype))
     return set_error(FD_ERR_INVALID, "prefill_workspace_size: bad sizes");
   *bytes = prefill_workspace_bytes(n, num_tokens, num_heads, num_kv_heads, head_size,
-                                   max_seqlen_q, max_keys, dtype);
+                                   max_seqlen_q, max_keys, block_size, dtype);
   return FD_OK;
 }
 

@@ -826,7 +826,7 @@ size_t balanced_partial_bytes(const SplitPlan& sp, int32_t H, int32_t D) {
 
 // 64-bit words from one of `pairs` arrival counters to the next: up to 256
 // bytes, as far as the caller's array reaches.
-static int32_t counter_stride(int64_t pairs) {
+int32_t counter_stride(int64_t pairs) {
   return (int32_t)std::min<int64_t>(32, kMaxBalPairs / std::max<int64_t>(pairs, 1));
 }
 
@@ -841,6 +841,18 @@ __global__ __launch_bounds__(256) void clear_counters_kernel(uint64_t* c, int32_
                                                              int32_t stride) {
   const int32_t k = blockIdx.x * 256 + threadIdx.x;
   if (k < count) c[k * stride] = 0;
+}
+
+int launch_clear_counters(uint64_t* c, int32_t count, int32_t stride, hipStream_t s) {
+  hipLaunchKernelGGL(clear_counters_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s,
+                     c, count, stride);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? FD_OK : hip_error(e, "clear_counters_kernel launch");
+}
+
+uint64_t next_launch() {
+  static std::atomic<uint64_t> launches{0};
+  return ++launches;
 }
 
 int launch_decode(const DecodeArgs& a, const SplitPlan& sp, hipStream_t s) {
@@ -948,18 +960,16 @@ int launch_decode(const DecodeArgs& a, const SplitPlan& sp, hipStream_t s) {
     tp.host_wgs = sp.host_wgs;
     tp.order = a.order;
     tp.wave_blocks = 0;
-    static std::atomic<uint64_t> launches{0};
-    tp.launch = ++launches << kArrivalBits;
+    static_assert(kArrivalBits == kLaunchBits, "numbered with the other launches");
+    tp.launch = next_launch() << kArrivalBits;
     tp.counters = a.counters;
     const int32_t count = a.n * a.KVH * sp.passes;
     tp.counter_stride = counter_stride(count);
     if (tp.counters == nullptr) {
       tp.counters = reinterpret_cast<uint64_t*>(static_cast<char*>(a.workspace) +
                                                 balanced_partial_bytes(sp, a.H, a.D));
-      hipLaunchKernelGGL(clear_counters_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256),
-                         0, s, tp.counters, count, tp.counter_stride);
-      const hipError_t e = hipGetLastError();
-      if (e != hipSuccess) return hip_error(e, "clear_counters_kernel launch");
+      const int rc = launch_clear_counters(tp.counters, count, tp.counter_stride, s);
+      if (rc != FD_OK) return rc;
     }
   } else if (sp.max_splits > 1) {
     char* ws = static_cast<char*>(a.workspace);

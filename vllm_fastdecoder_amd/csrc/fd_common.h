@@ -378,6 +378,14 @@ struct PlanTiersArgs {
 };
 int launch_plan_tiers(const PlanTiersArgs& a, hipStream_t s);
 
+// Arrival counters (decode_tiled.h, prefill_mm_kernel.h): launches that use
+// them are numbered together, kLaunchBits above the arrivals; count words,
+// stride apart, cleared by a kernel.
+constexpr int kLaunchBits = 24;
+uint64_t next_launch();
+int32_t counter_stride(int64_t count);
+int launch_clear_counters(uint64_t* c, int32_t count, int32_t stride, hipStream_t s);
+
 // Attention of packed query tokens (prefill.h): rows of several new tokens
 // over a paged cache (bt != NULL) or over packed keys and values.
 struct PrefillArgs {
@@ -403,12 +411,14 @@ struct PrefillArgs {
   float* lse;
   int64_t lse_sh;
   void* workspace;
+  uint64_t* counters;  // arrival counters (NULL: taken from the workspace and
+                       // cleared by a launch of their own)
 };
-int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s);
-// Workspace that a call of these sizes needs (kv_tokens: the longest row's
-// keys as far as the host knows).
+int launch_prefill(const PrefillArgs& a, hipStream_t s);
+// Workspace that a call of these sizes needs (max_k: the longest row's keys as
+// far as the host knows; BS: 0 for packed keys).
 size_t prefill_workspace_bytes(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_t D,
-                               int32_t max_q, int64_t max_k, int32_t dt);
+                               int32_t max_q, int64_t max_k, int32_t BS, int32_t dt);
 
 // Block tables, slot mapping, positions and lengths of a step (build_tables.hip).
 struct BuildTablesArgs {

@@ -51,54 +51,8 @@ int launch_prefill_generic(const PrefillArgs& a, hipStream_t s) {
   return e == hipSuccess ? FD_OK : hip_error(e, "prefill_generic_kernel launch");
 }
 
-// ------------------------------------------------------------ divided keys
+// ------------------------------------------------------------ the plan
 namespace {
-
-// The parts of a token and head's keys, joined: one wave each, lane l holding
-// elements 4 l .. + 3 (D = 256 in one go, smaller heads on fewer lanes).
-__global__ __launch_bounds__(256) void prefill_combine_kernel(PrefillMmParams p) {
-  const PrefillArgs& a = p.a;
-  const int lane = threadIdx.x % kWave;
-  const int64_t at = (int64_t)blockIdx.x * (256 / kWave) + threadIdx.x / kWave;
-  const int64_t all = (int64_t)a.T * a.H;
-  if (at >= all) return;
-  const int t = (int)(at / a.H), h = (int)(at % a.H);
-  const int i = last_row(a.n, t, [&](int r) { return (int64_t)a.cu_q[r]; });
-  const PrefillRow r = prefill_row(a, i);
-  if (t < r.q0 || t >= r.q0 + r.nq) return;
-  const bool small = (int64_t)r.nq * p.G <= kRowsB && p.plan.rows_b > 0;
-  const bool is_b = small || p.plan.tiles_a == 0;
-  const int parts = is_b ? p.plan.sb : p.plan.sa;
-  if (parts <= 1) return;  // written by its own workgroup
-  float m = neg_inf();
-  for (int s = lane; s < parts; s += kWave) m = fmaxf(m, p.part_ml[s * all + at].x);
-  m = wave_max(m);
-  const float base = m == neg_inf() ? 0.f : m;
-  float l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  const int d = 4 * lane;
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = p.part_ml[s * all + at];
-    if (ml.y == 0.f) continue;  // no key of this part is seen: nothing was stored
-    const float w = fast_exp2(ml.x - base);
-    l += w * ml.y;
-    if (d < a.D) {
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (s * all + at) * a.D + d);
-      acc.x += w * x.x;
-      acc.y += w * x.y;
-      acc.z += w * x.z;
-      acc.w += w * x.w;
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (lane == 0)
-    a.lse[(int64_t)h * a.lse_sh + t] = l == 0.f ? neg_inf() : (base + fast_log2(l)) * kLn2;
-  if (d >= a.D) return;
-  const int64_t o = (int64_t)t * a.out_st + (int64_t)h * a.out_sh + d;
-  const float y[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) store_elem(a.out, o + e, a.out_dt, y[e]);
-}
 
 int device_cu_count() {
   static thread_local int dev = -1, cus = 0;
@@ -119,52 +73,124 @@ int device_cu_count() {
   return cus;
 }
 
+// Keys of a step of the matrix-core kernel (PfShape).
+int64_t step_keys(int D, int dt) { return dtype_size(dt) * D <= 256 ? 64 : 32; }
+
+// Keys that lie one after another for certain, in a block of BS or (BS = 0)
+// packed, up to kMostRun, as a power of two.
+int run_shift(int BS) {
+  int s = 0;
+  while ((1 << s) < kMostRun && (BS == 0 || BS % (2 << s) == 0)) ++s;
+  return s;
+}
+
+int32_t prefill_counter_stride(int64_t pairs) {
+  return pairs <= kMaxPrefillCounters ? counter_stride(pairs) : 1;
+}
+
+// Into how many parts an A tile's keys are cut. A model of the time, in steps:
+// each part adds a start and an end, and parts are joined. Alike tiles (one
+// row) run in whole rounds; of different rows' tiles about half the work that
+// the longest row makes of them is there (the lengths are known on the GPU
+// alone), and three quarters of one part are waited for at the end. The start
+// and the join, from kernel traces: 12 to 18 and 10 us, a step 2.5 us (16-bit,
+// two workgroups on a CU; D = 256: 1.5, alone; fp32: 9). Measured, undivided /
+// as this divides / at its best: 4 chunks of 389 to 640 tokens over at most
+// 2048 keys, bf16 97 / 94 / 88 us; 3 of 200 to 700 over up to 4000, D = 256,
+// 121 / 101 / 101; 3 of 100 to 300 over up to 1500, fp32, 188 / 151 / 151.
+int64_t tile_parts(int n, int64_t tasks, int64_t steps, int64_t slots, int D, int dt) {
+  const double start = dt == FD_F32 ? 2 : D > 128 ? 10 : 7;
+  const double join = dt == FD_F32 ? 2 : D > 128 ? 12 : 6;
+  double least = 0, cost[kMostTileParts + 1];
+  const int64_t most = std::min<int64_t>(kMostTileParts, steps);
+  for (int64_t parts = 1; parts <= most; ++parts) {
+    const double part = (double)((steps + parts - 1) / parts) + start;
+    double& c = cost[parts];
+    if (n == 1) {
+      c = (double)((tasks * parts + slots - 1) / slots) * part;
+    } else {
+      const double work = 0.5 * (double)tasks * ((double)steps + (double)parts * start) / (double)slots;
+      c = std::max(part, work + 0.75 * part);
+    }
+    if (parts > 1) c += join;
+    least = parts == 1 ? c : std::min(least, c);
+  }
+  int64_t parts = 1;
+  while (cost[parts] > least * (1 + 1.0 / 32)) ++parts;  // the fewest of about as good
+  return parts;
+}
+
 bool mm_head_size(int D) { return (D % 16 == 0 && D >= 32 && D <= 128) || D == 256; }
 
 }  // namespace
 
-int launch_prefill_combine(const PrefillMmParams& p, hipStream_t s) {
-  const int64_t waves = (int64_t)p.a.T * p.a.H;
-  hipLaunchKernelGGL(prefill_combine_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, p);
-  const hipError_t e = hipGetLastError();
-  return e == hipSuccess ? FD_OK : hip_error(e, "prefill_combine_kernel launch");
-}
-
 PrefillPlan plan_prefill_mm(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_t D, int32_t max_q,
-                            int64_t max_k) {
+                            int64_t max_k, int32_t BS, int32_t dt) {
   PrefillPlan pl{};
   const int G = H / KVH;
   const int64_t rows = (int64_t)T * G;
   const int64_t longest = std::min<int64_t>(max_q, T) * G;
+  const int64_t keys = step_keys(D, dt);
+  const int64_t steps = std::max<int64_t>(1, (max_k + keys - 1) / keys);
+  const int64_t cus = device_cu_count();
+  // Eight waves where their tiles alone keep every CU busy for long: they
+  // read K and V half as often (bf16, 32 / 8 heads of 128, 4096 tokens over
+  // 28000 keys: 1874 us, with four waves 2326). Two workgroups of four share a
+  // CU, and one computes while the other starts or ends: better for short
+  // ones (16 fresh prompts of up to 512 tokens, 32 heads of 128: 52 us, with
+  // eight waves 62; four chunks of 389 to 640 tokens over at most 2048 keys:
+  // 97 and 115).
+  const int64_t wide = (rows + 255) / 256 * KVH;
+  pl.waves = D <= 128 && longest > kRowsB && steps >= 64 && wide >= (n == 1 ? cus : 2 * cus) ? 8 : 4;
+  const int rows_a = 32 * pl.waves;
   if (longest <= kRowsB) {
     pl.rows_b = n;
   } else if (n == 1) {
-    pl.tiles_a = (int32_t)((rows + kRowsA - 1) / kRowsA);
+    pl.tiles_a = (int32_t)((rows + rows_a - 1) / rows_a);
   } else {
     // a row among them may be of any size
     pl.rows_b = n;
-    pl.tiles_a = (int32_t)(rows / kRowsA + std::min<int64_t>(n, rows / (kRowsB + 1)));
+    pl.tiles_a = (int32_t)(rows / rows_a + std::min<int64_t>(n, rows / (kRowsB + 1)));
   }
-  // Keys are divided where there are fewer tasks than the CUs hold at once
-  // (two workgroups each).
-  const int64_t slots = 2LL * device_cu_count();
   const int64_t tasks = ((int64_t)pl.tiles_a + pl.rows_b) * KVH;
-  const int64_t steps = (max_k + 63) / 64;
-  const int64_t parts = std::max<int64_t>(1, std::min(slots / std::max<int64_t>(tasks, 1), steps / 4));
-  pl.sa = pl.tiles_a > 0 ? (int32_t)parts : 1;
-  pl.sb = pl.rows_b > 0 ? (int32_t)parts : 1;
-  if (parts > 1) pl.workspace = (size_t)parts * T * H * (D * sizeof(float) + sizeof(float2));
+  const int64_t slots = D > 128 || pl.waves == 8 ? cus : 2 * cus;  // workgroups at once
+  pl.per_a = pl.per_b = (int32_t)steps;
+  if (tasks <= kMaxPrefillCounters) {
+    const int64_t parts_a = tile_parts(n, tasks, steps, slots, D, dt);
+    pl.per_a = (int32_t)((steps + parts_a - 1) / parts_a);
+    // A row's few tokens, which its K and V's way from memory bounds: as many
+    // parts as run at once, of two steps at least (one row of 5 tokens, 900
+    // keys, 8 kv heads: 14.9 us, with parts of 1 step 16.2, of 4 17.1,
+    // undivided 26). Of many rows most are shorter than the longest: some more
+    // (48 rows of 2 to 9 tokens, up to 3100 keys, 4 kv heads: parts of 16
+    // steps 42 us, of 24 44, of 12 55, undivided 57).
+    const int64_t most = n == 1 ? slots : slots + slots / 4;
+    const int64_t parts = std::max<int64_t>(1, most / tasks);
+    pl.per_b = (int32_t)std::min(steps, std::max<int64_t>(2, (steps + parts - 1) / parts));
+  }
+  // a part's keys as far as their table has room
+  const int64_t most = ((int64_t)(kTableRoom - 2) << run_shift(BS)) / keys;
+  pl.per_a = (int32_t)std::min<int64_t>(pl.per_a, most);
+  pl.per_b = (int32_t)std::min<int64_t>(pl.per_b, most);
+  pl.parts_a = pl.tiles_a > 0 ? (int32_t)((steps + pl.per_a - 1) / pl.per_a) : 1;
+  pl.parts_b = pl.rows_b > 0 ? (int32_t)((steps + pl.per_b - 1) / pl.per_b) : 1;
+  const int64_t parts = std::max(pl.parts_a, pl.parts_b);
+  if (parts > 1) {
+    const size_t row = D * sizeof(float) + sizeof(float2);
+    pl.partial_bytes = ((size_t)parts * T * H * row + 255) / 256 * 256;
+    pl.counter_bytes = (size_t)tasks * prefill_counter_stride(tasks) * sizeof(uint64_t);
+  }
   return pl;
 }
 
 size_t prefill_workspace_bytes(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_t D,
-                               int32_t max_q, int64_t max_k, int32_t dt) {
+                               int32_t max_q, int64_t max_k, int32_t BS, int32_t dt) {
   if (!mm_head_size(D)) return 0;
-  return plan_prefill_mm(n, T, H, KVH, D, max_q, max_k).workspace;
+  const PrefillPlan pl = plan_prefill_mm(n, T, H, KVH, D, max_q, max_k, BS, dt);
+  return pl.partial_bytes + pl.counter_bytes;
 }
 
-int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s) {
-  (void)workspace_bytes;
+int launch_prefill(const PrefillArgs& a, hipStream_t s) {
   auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const int unit = a.dt == FD_F32 ? 4 : 8;  // elements of 16 bytes
   auto strides = [&](int64_t x, int64_t y) {
@@ -174,7 +200,8 @@ int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s) 
                     aligned(a.v) && aligned(a.out) && strides(a.q_st, a.q_sh) &&
                     strides(a.out_st, a.out_sh) && strides(a.k_st, a.k_sh) &&
                     strides(a.v_st, a.v_sh) && strides(a.k_sb, a.v_sb) &&
-                    (int64_t)a.max_q * (a.H / a.KVH) < (1 << 30) && a.max_k < INT32_MAX - 1024;
+                    (int64_t)a.T * (a.H / a.KVH) < (1 << 30) && a.max_k < INT32_MAX - 1024 &&
+                    std::max(a.k_st, a.v_st) < (1 << 30);
   if (!fast) return launch_prefill_generic(a, s);
   PrefillMmParams p{};
   p.a = a;
@@ -182,30 +209,39 @@ int launch_prefill(const PrefillArgs& a, size_t workspace_bytes, hipStream_t s) 
     p.a.k_sb = a.k_st;
     p.a.v_sb = a.v_st;
   }
-  p.plan = plan_prefill_mm(a.n, a.T, a.H, a.KVH, a.D, a.max_q, a.max_k);
+  p.plan = plan_prefill_mm(a.n, a.T, a.H, a.KVH, a.D, a.max_q, a.max_k,
+                           a.bt != nullptr ? a.BS : 0, a.dt);
+  const PrefillPlan& pl = p.plan;
   p.G = a.H / a.KVH;
   // (a scale of 0 makes all scores alike, which a scale too small to show does
   // too; its product with -inf, a masked score, is still -inf)
   const float scale = a.scale * kLog2e;
   p.q_flip = scale >= 0.f ? 0u : a.dt == FD_F32 ? 0x80000000u : 0x80008000u;
   p.scale_log2 = scale == 0.f ? 0x1p-100f : std::fabs(scale);
-  int sh = 0;
-  while ((1ll << sh) < a.BS) ++sh;
-  p.bs_shift = 31 + sh;
-  p.bs_magic = (uint32_t)(((1ull << (31 + sh)) + a.BS - 1) / a.BS);
-  if (p.plan.workspace > 0) {
-    const int parts = std::max(p.plan.sa, p.plan.sb);
+  const int64_t keys = step_keys(a.D, a.dt);
+  p.run_shift = run_shift(a.bt != nullptr ? a.BS : 0);
+  const int64_t per = std::max(pl.tiles_a > 0 ? pl.per_a : 0, pl.rows_b > 0 ? pl.per_b : 0);
+  p.table_room = (int32_t)(((per * keys) >> p.run_shift) + 2);
+  p.grid = ((int64_t)pl.tiles_a * pl.parts_a + (int64_t)pl.rows_b * pl.parts_b) * a.KVH;
+  if (p.grid > INT32_MAX) return set_error(FD_ERR_UNSUPPORTED, "prefill: too many tasks");
+  p.alone = p.grid <= device_cu_count();
+  if (pl.partial_bytes > 0) {
+    const int parts = std::max(pl.parts_a, pl.parts_b);
+    const int64_t pairs = ((int64_t)pl.tiles_a + pl.rows_b) * a.KVH;
     p.part_o = static_cast<float*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)parts * a.T * a.H * a.D);
+    p.counters = pairs <= kMaxPrefillCounters ? a.counters : nullptr;
+    p.counter_stride = prefill_counter_stride(pairs);
+    p.launch = next_launch() << kLaunchBits;
+    if (p.counters == nullptr) {
+      p.counters = reinterpret_cast<uint64_t*>(static_cast<char*>(a.workspace) + pl.partial_bytes);
+      const int rc = launch_clear_counters(p.counters, (int32_t)pairs, p.counter_stride, s);
+      if (rc != FD_OK) return rc;
+    }
   }
-  const int64_t tasks =
-      ((int64_t)p.plan.tiles_a * p.plan.sa + (int64_t)p.plan.rows_b * p.plan.sb) * a.KVH;
-  if (tasks > INT32_MAX) return set_error(FD_ERR_UNSUPPORTED, "prefill: too many tasks");
-  const int rc = a.dt == FD_F16    ? launch_prefill_mm_f16(p, s)
-                 : a.dt == FD_BF16 ? launch_prefill_mm_bf16(p, s)
-                                   : launch_prefill_mm_f32(p, s);
-  if (rc != FD_OK || (p.plan.sa <= 1 && p.plan.sb <= 1)) return rc;
-  return launch_prefill_combine(p, s);
+  return a.dt == FD_F16    ? launch_prefill_mm_f16(p, s)
+         : a.dt == FD_BF16 ? launch_prefill_mm_bf16(p, s)
+                           : launch_prefill_mm_f32(p, s);
 }
 
 }  // namespace fd

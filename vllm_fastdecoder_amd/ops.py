@@ -982,17 +982,18 @@ _PREFILL_WS_SIZES: dict = {}
 
 
 def prefill_workspace_bytes(n: int, num_tokens: int, H: int, KVH: int, D: int, max_seqlen_q: int,
-                            max_keys: int, dtype: torch.dtype) -> int:
+                            max_keys: int, block_size: int, dtype: torch.dtype) -> int:
     """Workspace a paged_prefill (max_keys: its table's columns times the block
-    size) or varlen_attention (max_keys: max_seqlen_k) call of these sizes
+    size) or varlen_attention (max_keys: max_seqlen_k, block_size 0) call of these sizes
     needs on the current device (fd_prefill_workspace_size, remembered). For
     reserve_workspace ahead of a graph capture."""
-    key = (n, num_tokens, H, KVH, D, max_seqlen_q, max_keys, dtype, _current_device())
+    key = (n, num_tokens, H, KVH, D, max_seqlen_q, max_keys, block_size, dtype, _current_device())
     size = _PREFILL_WS_SIZES.get(key)
     if size is None:
         c = ctypes.c_size_t()
         _lib.check(_lib.load_lib().fd_prefill_workspace_size(n, num_tokens, H, KVH, D,
-                                                             max_seqlen_q, max_keys, _DT[dtype],
+                                                             max_seqlen_q, max_keys, block_size,
+                                                             _DT[dtype],
                                                              ctypes.byref(c)))
         size = int(c.value)
         if len(_PREFILL_WS_SIZES) > 4096:
@@ -1082,7 +1083,7 @@ def paged_prefill(
     ln = _on_device(seqused_k, dev).contiguous()
     cu = _on_device(cu_seqlens_q, dev).contiguous()
     ws = WORKSPACE.get(dev, prefill_workspace_bytes(n, T, H, KVH, D, int(max_seqlen_q), W * BS,
-                                                    q.dtype))
+                                                    BS, q.dtype))
     _launch(dev, _lib.load_lib().fd_paged_prefill,
             q.data_ptr(), q.stride(0), q.stride(1), device_ptr(key_cache), device_ptr(value_cache),
             key_cache.stride(0), key_cache.stride(2), key_cache.stride(1), B,
@@ -1091,7 +1092,7 @@ def paged_prefill(
             float(softmax_scale), _DT[q.dtype], out.data_ptr(), out.stride(0), out.stride(1),
             _DT[out.dtype], lse.data_ptr(), lse.stride(0),
             ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            _stream_for(q))
+            _stream_for(q), _counters_ptr(ws))
     return out, lse
 
 
@@ -1131,7 +1132,7 @@ def varlen_attention(
     cu = _on_device(cu_seqlens_q, dev).contiguous()
     cuk = _on_device(cu_seqlens_k, dev).contiguous()
     ws = WORKSPACE.get(dev, prefill_workspace_bytes(n, T, H, KVH, D, int(max_seqlen_q),
-                                                    int(max_seqlen_k), q.dtype))
+                                                    int(max_seqlen_k), 0, q.dtype))
     _launch(dev, _lib.load_lib().fd_varlen_attention,
             q.data_ptr(), q.stride(0), q.stride(1), device_ptr(k), k.stride(0), k.stride(1),
             device_ptr(v), v.stride(0), v.stride(1), cu.data_ptr(), cuk.data_ptr(), n, T,
@@ -1139,7 +1140,7 @@ def varlen_attention(
             float(softmax_scale), _DT[q.dtype], out.data_ptr(), out.stride(0), out.stride(1),
             _DT[out.dtype], lse.data_ptr(), lse.stride(0),
             ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-            _stream_for(q))
+            _stream_for(q), _counters_ptr(ws))
     return out, lse
 
 
