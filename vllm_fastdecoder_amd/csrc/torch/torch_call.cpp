@@ -1,5 +1,6 @@
-// The ordinary form of ops.paged_decode and of the cache writes taken from
-// torch tensors straight to the C ABI, in one native call.
+// The ordinary form of ops.paged_decode, of the attention of packed tokens, of
+// the step tables and of the cache writes taken from torch tensors straight to
+// the C ABI, in one native call.
 //
 // What bounds a small launch is the host: through ctypes a decode call took
 // 13-15 us (about forty attribute reads and checks in Python, two tensor
@@ -20,6 +21,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <torch/csrc/Device.h>
@@ -85,6 +87,27 @@ bool to_int64(PyObject* o, int64_t* out) {
 }
 
 bool fits32(int64_t x) { return x >= 0 && x <= INT32_MAX; }
+
+// An int of 0 .. INT32_MAX.
+bool to_int32(PyObject* o, int32_t* out) {
+  int64_t x;
+  if (!to_int64(o, &x) || !fits32(x)) return false;
+  *out = (int32_t)x;
+  return true;
+}
+
+bool on_current_device(const at::Tensor& t) {
+  return c10::impl::getDeviceGuardImpl(at::kCUDA)->getDevice().index() == t.get_device();
+}
+
+// An int32 [size] on t's device.
+const int32_t* index_row(const at::Tensor& t, PyObject* o, int64_t size) {
+  const at::Tensor* x = plain_gpu(o, at::kInt);
+  if (x == nullptr || x->dim() != 1 || x->size(0) != size || !x->is_contiguous() ||
+      x->device() != t.device())
+    return nullptr;
+  return x->data_ptr<int32_t>();
+}
 
 // Calls that torch modes would have to see go through Python.
 bool modes_active() {
@@ -297,6 +320,125 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
+// What paged_prefill and varlen_attention share: q [T, H, D], k and v of dims
+// [.., KVH, D], the rows' starts.
+struct Packed {
+  const at::Tensor *q, *k, *v;
+  const int32_t* cu;
+  int32_t n, T, H, KVH, D, max_q, causal;
+  bool ok = false;
+  Packed(PyObject* q_o, PyObject* k_o, PyObject* v_o, int64_t dims, PyObject* cu_o,
+         PyObject* scale_o, PyObject* max_q_o, PyObject* causal_o)
+      : q(query(q_o)), k(plain(k_o)), v(plain(v_o)) {
+    if (q == nullptr || k == nullptr || v == nullptr || !k->is_cuda() || !v->is_cuda() ||
+        k->device() != q->device() || v->device() != q->device() || k->dim() != dims ||
+        !k->sizes().equals(v->sizes()) || k->scalar_type() != q->scalar_type() ||
+        v->scalar_type() != q->scalar_type() || k->stride(dims - 1) != 1 ||
+        v->stride(dims - 1) != 1 || k->size(dims - 1) != q->size(2) || !on_current_device(*q) ||
+        !fits32(q->size(1)) || !fits32(q->size(2)) || !fits32(k->size(dims - 2)) ||
+        !PyFloat_CheckExact(scale_o) || !PyBool_Check(causal_o) || !to_int32(max_q_o, &max_q))
+      return;
+    const at::Tensor* c = plain_gpu(cu_o, at::kInt);
+    if (c == nullptr || c->dim() != 1 || c->size(0) < 2 || !fits32(c->size(0))) return;
+    T = (int32_t)q->size(0);
+    H = (int32_t)q->size(1);
+    D = (int32_t)q->size(2);
+    KVH = (int32_t)k->size(dims - 2);
+    n = (int32_t)c->size(0) - 1;
+    causal = causal_o == Py_True;
+    cu = index_row(*q, cu_o, c->size(0));
+    ok = cu != nullptr && H > 0 && D > 0 && KVH > 0 && H % KVH == 0;
+  }
+  // (contiguous, whatever q's strides are)
+  void allocate(Outputs& o) const {
+    if (!o.out.defined()) o.out = at::empty(q->sizes(), q->options());
+    if (!o.lse.defined()) o.lse = at::empty({H, T}, q->options().dtype(at::kFloat));
+  }
+};
+
+// paged_prefill(q, key_cache, value_cache, block_table, cu_seqlens_q,
+//               seqused_k, scale, max_seqlen_q, max_seqlen_k, causal, out, lse)
+PyObject* paged_prefill(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    if (na != 12 || modes_active()) return not_here();
+    const Packed x(a[0], a[1], a[2], 4, a[4], a[6], a[7], a[9]);
+    const at::Tensor* bt = plain_gpu(a[3], at::kInt);
+    if (!x.ok || !same_layout(*x.k, *x.v) || bt == nullptr || bt->dim() != 2 ||
+        bt->size(0) != x.n || bt->size(1) <= 0 || bt->stride(1) != 1 || !fits32(bt->size(1)) ||
+        bt->device() != x.q->device())
+      return not_here();
+    const int32_t* lens = index_row(*x.q, a[5], x.n);
+    const int64_t BS = x.k->size(1);
+    if (lens == nullptr || BS == 0 || !fits32(BS)) return not_here();
+    int64_t width = bt->size(1);
+    if (a[8] != Py_None) {
+      int32_t longest;
+      if (!to_int32(a[8], &longest)) return not_here();
+      width = std::min(width, std::max<int64_t>(1, (longest + BS - 1) / BS));
+    }
+    Outputs o(*x.q, a[10], a[11]);
+    if (!o.ok) return not_here();
+    const int kv = dtype_code(x.q->scalar_type());
+    size_t need = 0;
+    if (fd_prefill_workspace_size(x.n, x.T, x.H, x.KVH, x.D, x.max_q, width * BS, (int32_t)BS, kv,
+                                  &need) != FD_OK)
+      return not_here();
+    x.allocate(o);
+    PyRef hold;
+    void *ws, *stream;
+    size_t ws_bytes;
+    uint32_t* counters;
+    if (!current_stream(x.q->get_device(), &stream) ||
+        !workspace(*x.q, need, stream, hold, &ws, &ws_bytes, &counters))
+      return nullptr;
+    const float scale = (float)PyFloat_AS_DOUBLE(a[6]);
+    const int64_t bt_stride = x.n == 1 ? std::max(bt->stride(0), width) : bt->stride(0);
+    const int status = without_gil([&] { return fd_paged_prefill(
+        x.q->data_ptr(), x.q->stride(0), x.q->stride(1), x.k->data_ptr(), x.v->data_ptr(),
+        x.k->stride(0), x.k->stride(2), x.k->stride(1), x.k->size(0), bt->data_ptr<int32_t>(),
+        bt_stride, (int32_t)width, x.cu, lens, x.n, x.T, x.max_q, x.causal, x.H, x.KVH, x.D,
+        (int32_t)BS, scale, kv, o.out.data_ptr(), o.out.stride(0), o.out.stride(1),
+        dtype_code(o.out.scalar_type()), o.lse.data_ptr<float>(), o.lse.stride(0), ws, ws_bytes,
+        stream, counters); });
+    return result(status, o);
+  });
+}
+
+// varlen_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, scale, max_seqlen_q,
+//                  max_seqlen_k, causal, out, lse)
+PyObject* varlen_attention(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    if (na != 11 || modes_active()) return not_here();
+    const Packed x(a[0], a[1], a[2], 3, a[3], a[5], a[6], a[8]);
+    int32_t max_k;
+    if (!x.ok || !to_int32(a[7], &max_k) || !fits32(x.k->size(0))) return not_here();
+    const int32_t* cu_k = index_row(*x.q, a[4], (int64_t)x.n + 1);
+    Outputs o(*x.q, a[9], a[10]);
+    if (cu_k == nullptr || !o.ok) return not_here();
+    const int kv = dtype_code(x.q->scalar_type());
+    size_t need = 0;
+    if (fd_prefill_workspace_size(x.n, x.T, x.H, x.KVH, x.D, x.max_q, max_k, 0, kv, &need) !=
+            FD_OK)
+      return not_here();
+    x.allocate(o);
+    PyRef hold;
+    void *ws, *stream;
+    size_t ws_bytes;
+    uint32_t* counters;
+    if (!current_stream(x.q->get_device(), &stream) ||
+        !workspace(*x.q, need, stream, hold, &ws, &ws_bytes, &counters))
+      return nullptr;
+    const float scale = (float)PyFloat_AS_DOUBLE(a[5]);
+    const int status = without_gil([&] { return fd_varlen_attention(
+        x.q->data_ptr(), x.q->stride(0), x.q->stride(1), x.k->data_ptr(), x.k->stride(0),
+        x.k->stride(1), x.v->data_ptr(), x.v->stride(0), x.v->stride(1), x.cu, cu_k, x.n, x.T,
+        (int32_t)x.k->size(0), x.max_q, max_k, x.causal, x.H, x.KVH, x.D, scale, kv,
+        o.out.data_ptr(), o.out.stride(0), o.out.stride(1), dtype_code(o.out.scalar_type()),
+        o.lse.data_ptr<float>(), o.lse.stride(0), ws, ws_bytes, stream, counters); });
+    return result(status, o);
+  });
+}
+
 // key and value rows [T, KVH, D] of one shape, T given by the slots.
 bool kv_rows(const at::Tensor* key, const at::Tensor* value) {
   return key != nullptr && value != nullptr && key->is_cuda() && value->device() == key->device() &&
@@ -400,6 +542,59 @@ PyObject* cache_write_tiers(PyObject*, PyObject* const* a, Py_ssize_t na) {
   });
 }
 
+// build_tables(query_start_loc, context_lens, block_table, block_size,
+//              num_tokens, num_blocks, free_blocks, taken, error_count)
+//   -> (slot_mapping, positions, seq_lens, taken or None), or (status,)
+PyObject* build_tables(PyObject*, PyObject* const* a, Py_ssize_t na) {
+  return guarded([&]() -> PyObject* {
+    if (na != 9 || modes_active()) return not_here();
+    const at::Tensor* bt = plain_gpu(a[2], at::kInt);
+    int32_t BS, T;
+    int64_t blocks;
+    if (bt == nullptr || bt->dim() != 2 || bt->size(0) <= 0 || bt->size(1) <= 0 ||
+        bt->stride(1) != 1 || (bt->size(0) > 1 && bt->stride(0) < bt->size(1)) ||
+        !fits32(bt->size(0)) || !fits32(bt->size(1)) || !on_current_device(*bt) ||
+        !to_int32(a[3], &BS) || BS == 0 || !to_int32(a[4], &T) || !to_int64(a[5], &blocks) ||
+        blocks < 0)
+      return not_here();
+    const int64_t n = bt->size(0), W = bt->size(1);
+    const int32_t* starts = index_row(*bt, a[0], n + 1);
+    const int32_t* held = index_row(*bt, a[1], n);
+    int32_t* errors;
+    if (starts == nullptr || held == nullptr || !device_counter(a[8], &errors) ||
+        (errors != nullptr && THPVariable_Unpack(a[8]).device() != bt->device()) ||
+        (a[6] == Py_None) != (a[7] == Py_None))
+      return not_here();
+    const int32_t *free_ids = nullptr, *taken = nullptr;
+    int64_t num_free = 0;
+    at::Tensor taken_out;
+    if (a[6] != Py_None) {
+      const at::Tensor* f = plain_gpu(a[6], at::kInt);
+      if (f == nullptr || f->dim() != 1 || f->size(0) <= 0 || !fits32(f->size(0))) return not_here();
+      num_free = f->size(0);
+      free_ids = index_row(*bt, a[6], num_free);
+      taken = index_row(*bt, a[7], 1);
+      if (free_ids == nullptr || taken == nullptr) return not_here();
+      taken_out = at::empty({1}, bt->options());
+    }
+    const at::Tensor slots = at::empty({T}, bt->options().dtype(at::kLong));
+    const at::Tensor positions = at::empty({T}, bt->options().dtype(at::kLong));
+    const at::Tensor seq_lens = at::empty({n}, bt->options());
+    void* stream;
+    if (!current_stream(bt->get_device(), &stream)) return nullptr;
+    const int status = without_gil([&] { return fd_build_tables(
+        starts, held, (int32_t)n, T, BS, bt->data_ptr<int32_t>(), n > 1 ? bt->stride(0) : W,
+        (int32_t)W, blocks, free_ids, (int32_t)num_free, taken,
+        taken_out.defined() ? taken_out.data_ptr<int32_t>() : nullptr, slots.data_ptr<int64_t>(),
+        positions.data_ptr<int64_t>(), seq_lens.data_ptr<int32_t>(), errors, stream); });
+    if (status != FD_OK) return Py_BuildValue("(i)", status);
+    PyRef s(THPVariable_Wrap(slots)), p(THPVariable_Wrap(positions)), l(THPVariable_Wrap(seq_lens));
+    PyRef t(taken_out.defined() ? THPVariable_Wrap(taken_out) : Py_NewRef(Py_None));
+    if (s.p == nullptr || p.p == nullptr || l.p == nullptr || t.p == nullptr) return nullptr;
+    return PyTuple_Pack(4, s.p, p.p, l.p, t.p);
+  });
+}
+
 // init(WORKSPACE.get, pinned.device_ptr, raw current-stream query,
 //      torch.__version__): an ImportError where the module was built against
 // another torch, whose tensors it would read by the wrong layout, or beside a
@@ -426,6 +621,13 @@ PyObject* init(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"init", init, METH_VARARGS, nullptr},
     {"paged_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_decode)),
+     METH_FASTCALL, nullptr},
+    {"paged_prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_prefill)),
+     METH_FASTCALL, nullptr},
+    {"varlen_attention",
+     reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(varlen_attention)), METH_FASTCALL,
+     nullptr},
+    {"build_tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(build_tables)),
      METH_FASTCALL, nullptr},
     {"cache_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_write)),
      METH_FASTCALL, nullptr},

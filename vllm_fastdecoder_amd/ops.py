@@ -1059,6 +1059,12 @@ def paged_prefill(
     outside the cache: its out and lse are NaN. Returns out [T, H, D] (q's
     dtype unless given) and lse [H, T] float32; a token without keys gives 0
     and -inf, tokens in no row are not written."""
+    native = _NATIVE or _native()
+    if native:
+        got = native.paged_prefill(q, key_cache, value_cache, block_table, cu_seqlens_q, seqused_k,
+                                   softmax_scale, max_seqlen_q, max_seqlen_k, causal, out, lse)
+        if got is not None:
+            return _native_result(got)
     _require(key_cache.dim() == 4 and value_cache.shape == key_cache.shape
              and key_cache.stride() == value_cache.stride(),
              "key_cache/value_cache must be [B, BS, KVH, D] of one shape and strides")
@@ -1120,6 +1126,12 @@ def varlen_attention(
     0 .. k_i - q_i + j. max_seqlen_q / max_seqlen_k as for paged_prefill.
     Returns out [T, H, D] and lse [H, T] float32; a token without keys gives 0
     and -inf, tokens in no row are not written."""
+    native = _NATIVE or _native()
+    if native:
+        got = native.varlen_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, softmax_scale,
+                                      max_seqlen_q, max_seqlen_k, causal, out, lse)
+        if got is not None:
+            return _native_result(got)
     _require(k.dim() == 3, "k and v must be [Tk, KVH, D]")
     T, H, D, KVH, n, out, lse = _prefill_args(q, k, v, cu_seqlens_q, max_seqlen_q, out, lse)
     _require(cu_seqlens_k.dtype == torch.int32 and cu_seqlens_k.shape == (n + 1,),
@@ -1170,6 +1182,12 @@ def build_tables(
     (slot_mapping int64 [num_tokens], positions int64 [num_tokens], seq_lens
     int32 [n], the new count of taken blocks or None). error_count: int32 [1]
     GPU counter of rows and tokens that got no slot (see include/fdattn.h)."""
+    native = _NATIVE or _native()
+    if native:
+        got = native.build_tables(query_start_loc, context_lens, block_table, block_size,
+                                  num_tokens, num_blocks, free_blocks, taken, error_count)
+        if got is not None:
+            return _native_result(got)
     _require(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2,
              "block_table must be int32 [n, W] on the GPU")
     n, W = block_table.shape
