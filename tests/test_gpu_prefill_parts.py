@@ -143,6 +143,22 @@ def test_more_tasks_than_counters(gpu):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("qs,ks", [([40] * 30, [6500] * 2 + [9] * 28), ([3], [6500])], ids=["chunks", "one"])
+def test_tables_as_long_as_they_get(gpu, dtype, D, qs, ks):
+    """Single-token blocks, a place looked up for every key, beside the largest stages."""
+    qs = [min(q, k) for q, k in zip(qs, ks)]
+    p = po.Paged(qs, ks, 16, 16, D, dtype, BS=1, seed=36)
+    out, lse = _run(p)
+    rows = [(0, 0), (sum(qs[:-1]), len(qs) - 1)]
+    for q0, i in rows:
+        for h in (0, 15):
+            q = p.q[q0:q0 + qs[i], h:h + 1]
+            ref = po.attend(q, p.k[i][:, h:h + 1], p.v[i][:, h:h + 1], 0.125, True, out.dtype)
+            po.check(out[q0:q0 + qs[i], h:h + 1], lse[h:h + 1, q0:q0 + qs[i]], ref, f"row {i} head {h}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_without_arrival_counters(gpu, dtype, monkeypatch):
     """A caller that gives no counters: they lie in the workspace, and a graph clears them."""
     monkeypatch.setattr(ops, "_counters_ptr", lambda *a, **k: None)

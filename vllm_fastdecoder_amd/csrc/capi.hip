@@ -742,7 +742,8 @@ int fd_prefill_workspace_size(int32_t n, int32_t num_tokens, int32_t num_heads,
       block_size < 0 || !valid_dtype(dtype))
     return set_error(FD_ERR_INVALID, "prefill_workspace_size: bad sizes");
   *bytes = prefill_workspace_bytes(n, num_tokens, num_heads, num_kv_heads, head_size,
-                                   max_seqlen_q, max_keys, block_size, dtype);
+                                   max_seqlen_q, std::min<int64_t>(max_keys, INT32_MAX), block_size,
+                                   dtype);
   return FD_OK;
 }
 

@@ -76,6 +76,13 @@ int device_cu_count() {
 // Keys of a step of the matrix-core kernel (PfShape).
 int64_t step_keys(int D, int dt) { return dtype_size(dt) * D <= 256 ? 64 : 32; }
 
+// Runs that a part's table has room for: with V's own beside K's, two stages of
+// K and V fit the LDS too.
+int64_t table_room(int D, int dt) {
+  const int64_t stage = 2 * step_keys(D, dt) * D * (int64_t)dtype_size(dt);
+  return std::min<int64_t>(kTableRoom, (kPrefillLds - 2 * stage) / 16);
+}
+
 // Keys that lie one after another for certain, in a block of BS or (BS = 0)
 // packed, up to kMostRun, as a power of two.
 int run_shift(int BS) {
@@ -169,7 +176,7 @@ PrefillPlan plan_prefill_mm(int32_t n, int32_t T, int32_t H, int32_t KVH, int32_
     pl.per_b = (int32_t)std::min(steps, std::max<int64_t>(2, (steps + parts - 1) / parts));
   }
   // a part's keys as far as their table has room
-  const int64_t most = ((int64_t)(kTableRoom - 2) << run_shift(BS)) / keys;
+  const int64_t most = ((int64_t)(table_room(D, dt) - 2) << run_shift(BS)) / keys;
   pl.per_a = (int32_t)std::min<int64_t>(pl.per_a, most);
   pl.per_b = (int32_t)std::min<int64_t>(pl.per_b, most);
   pl.parts_a = pl.tiles_a > 0 ? (int32_t)((steps + pl.per_a - 1) / pl.per_a) : 1;

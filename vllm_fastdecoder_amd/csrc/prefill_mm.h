@@ -22,7 +22,8 @@ struct PrefillPlan {
 constexpr int kRowsB = 64;
 constexpr int kMostTileParts = 32;   // of an A tile's keys
 constexpr int kMostRun = 16;         // keys whose place is looked up as one, at most
-constexpr int kTableRoom = 4096;     // runs of a part (32 KiB of LDS; twice that if V's differ)
+constexpr int kTableRoom = 4096;     // runs of a part at most (32 KiB of LDS; twice that if V's differ)
+constexpr int kPrefillLds = 155 * 1024;    // of a workgroup, for its stages and tables
 constexpr int kMaxPrefillCounters = 2048;  // 64-bit words of the caller's FD_DECODE_COUNTERS
 
 struct PrefillMmParams {

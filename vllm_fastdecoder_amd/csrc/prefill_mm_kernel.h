@@ -974,6 +974,7 @@ hipError_t launch_d(PrefillMmParams p, hipStream_t s) {
   const bool two = NW == 4 && Shape::kWavesPerSimd == 2 && half >= 2 && !p.alone;
   const int per = std::max(p.plan.tiles_a > 0 ? p.plan.per_a : 0, p.plan.rows_b > 0 ? p.plan.per_b : 0);
   p.stages = std::min(std::min(4, std::max(2, per + 1)), two ? half : (kMost - tail) / Shape::kStageBytes);
+  if (p.stages < 2) return hipErrorInvalidValue;  // (table_room in prefill.hip leaves room for two)
   hipLaunchKernelGGL(kernel, dim3((unsigned)p.grid), dim3(Shape::kThreads),
                      p.stages * Shape::kStageBytes + tail, s, p);
   return hipGetLastError();
