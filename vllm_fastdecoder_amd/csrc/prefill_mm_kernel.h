@@ -47,14 +47,16 @@
 // that it sees.
 //
 // What bounds it (bf16, 32 / 8 heads of 128): the wave's own issue of
-// instructions. A step of a wave is 1024 cycles of matrix instructions and about
-// 470 issue slots of the rest (counters: 294 VALU instructions, most of them
-// the softmax's exponents, sums and conversions, and LDS reads), which overlap
-// only as far as the two waves of a SIMD are in different phases. 8 waves, 4096
-// tokens over 28000 keys: 1874 us, 1.08 PFLOP/s (a large matrix product reaches
-// 1.20); with every operand read right ahead of its product and no work beside
-// it the same took 2331 us, with the weights computed after the scores' products
-// 2078. D = 256: 0.81 PFLOP/s (one wave a SIMD); fp32: 0.130 of 0.153.
+// instructions. A step of a wave is 1024 cycles of matrix instructions beside
+// about 260 VALU instructions (32 exponents, sums, fmas for the exponents, 16
+// conversions and maxima of three, the loads' addresses) and 48 LDS reads,
+// which overlap only as far as the two waves of a SIMD are in different phases.
+// 8 waves, 4096 tokens over 28000 keys: 1815 us, 1.11 PFLOP/s (a large matrix
+// product reaches 1.20). The same with every operand read right ahead of its
+// product 2331 us; with the weights computed between the two products 2078; with
+// scores copied, then turned into exponents as the weights are made (32 VALU
+// instructions more) 1900. D = 256: 0.8 PFLOP/s (one wave a SIMD); fp32: 0.130 of
+// 0.153.
 #pragma once
 
 #include <algorithm>
@@ -435,9 +437,9 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, const PfTask& 
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[db][e] = 0.f;
 
-  f32x16 s[NB];   // the step's scores, then (fp32) its weights
+  f32x16 s[NB];   // the step's weights' exponents, then (fp32) its weights
   f32x16 sn[NB];  // the next step's scores
-  f32x16 sw[NB];  // the same, on their way to s
+  f32x16 sw[NB];  // the next step's exponents, on their way to s
   // scores of the K in `ks_lds`, with `beside` going on
   u32x4 buf[AHEAD];
   auto scores = [&](const char* ks_lds, auto&& beside, auto&& next) {
@@ -495,27 +497,37 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, const PfTask& 
         sn[nb][e] = key <= vis ? sn[nb][e] : neg_inf();
       }
   };
+  float ms = -kShift;  // what the exponents are relative to: the running maximum, less the shift
   float top = 0.f;
-  // part x of n of taking the next step's scores over (their maximum first)
+  // part x of n of the next step's exponents, by the maximum so far, and their
+  // own maximum
   auto take = [&](int x, int n) {
 #pragma unroll
     for (int e = 16 * NB * x / n; e < 16 * NB * (x + 1) / n; ++e) {
-      float y = sn[e / 16][e % 16];
-      top = e == 0 ? y : fmaxf(top, y);
+      float y = fmaf(sn[e / 16][e % 16], p.scale_log2, -ms);
       stay(y);
+      top = e == 0 ? y : fmaxf(top, y);
       sw[e / 16][e % 16] = y;
     }
     stay(top);
   };
-  // the running maximum, raised where they pass it by too much
+  // the running maximum, raised where they pass it by too much (seldom: only
+  // then are the exponents moved, and what is summed rescaled)
   auto raise_max = [&]() {
-    top = xor_max<32>(top) * p.scale_log2;
-    const bool raise = top > m + kLazyRescale;  // false while both are -inf
+    top = xor_max<32>(top);
+    // (the first keys raise it whatever they score; -inf is none)
+    const bool raise = top > (m == neg_inf() ? neg_inf() : kLazyRescale + kShift);
     if (__ballot(raise) != 0) {
-      const float mn = raise ? top : m;
+      const float mn = raise ? top + ms : m;
       const float alpha = raise ? fast_exp2(m - mn) : 1.f;
+      const float by = raise ? (mn - kShift) - ms : 0.f;  // the exponents' move
       m = mn;
+      ms = raise ? mn - kShift : ms;
       l *= alpha;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sw[nb][e] -= by;
 #pragma unroll
       for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -523,7 +535,7 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, const PfTask& 
     }
   };
   u32x4 pf[F ? 1 : 2 * NB];
-  float ms = 0.f, sum[2];
+  float sum[2];
   // pair x of the step's weights
   auto weights = [&](int x) {
     const int nb = x / 8, e = x % 8 * 2;
@@ -531,7 +543,7 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, const PfTask& 
     for (int k = 0; k < 2; ++k) {
       float y = s[nb][e + k];
       stay(y);
-      y = fast_exp2(fmaf(y, p.scale_log2, -ms));
+      y = fast_exp2(y);
       sum[k] += y;
       if constexpr (F) stay(y);
       s[nb][e + k] = y;
@@ -574,7 +586,6 @@ __device__ __forceinline__ bool pf_tile(const PrefillMmParams& p, const PfTask& 
     const bool beside = more && whole(step + stages - 1);
     if (!beside && step + stages - 1 < s_to) load_last(wr, step + stages - 1, 1);
     if (step < w_to) {
-      ms = (m == neg_inf() ? 0.f : m) - kShift;
       sum[0] = sum[1] = 0.f;
       auto next_value = [&](int y) { return value(vs_lds, y); };
       auto some_weights = [&](int x) {
