@@ -48,8 +48,8 @@
 //
 // What bounds it (bf16, 32 / 8 heads of 128): the wave's own issue of
 // instructions. A step of a wave is 1024 cycles of matrix instructions beside
-// about 190 VALU instructions (32 exponents, sums, fmas for the exponents, 16
-// conversions and maxima of three, the loads' addresses) and 48 LDS reads,
+// about 210 VALU instructions (32 exponents, sums, fmas for the exponents, 16
+// conversions and maxima of three, the loads' addresses) and 52 LDS instructions,
 // which overlap only as far as the two waves of a SIMD are in different phases.
 // 8 waves, 4096 tokens over 28000 keys: 1815 us, 1.11 PFLOP/s (a large matrix
 // product reaches 1.20). The same with every operand read right ahead of its
