@@ -10,6 +10,7 @@ import torch
 
 from tests import prefill_oracle as po
 from vllm_fastdecoder_amd import ops
+from vllm_fastdecoder_amd.pinned import pinned_zeros
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +184,60 @@ def test_without_arrival_counters(gpu, dtype, monkeypatch):
         assert torch.equal(out, eager[0]) and torch.equal(lse, eager[1])
         call()
     ops.release_workspace(side)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 72])
+def test_a_cache_in_pinned_host_memory(gpu, dtype, D):
+    """The host tier's own layout, read in place."""
+    p = po.Paged([40, 2], [300, 900], 4, 2, D, dtype, seed=37)
+    k, v = (pinned_zeros((p.B, 2, p.BS, D), dtype) for _ in range(2))
+    k.copy_(p.kv[..., :D].transpose(1, 2))
+    v.copy_(p.kv[..., D:].transpose(1, 2))
+    _check(p, *_run(p, k=k.transpose(1, 2), v=v.transpose(1, 2)))
+
+
+def test_output_over_the_queries(gpu):
+    """Every tile reads its own queries only, and before it writes."""
+    p = po.Paged([130, 3], [2000, 1000], 8, 2, 64, torch.bfloat16, seed=38)
+    kv, q = p.kv.to(gpu), p.q.to(gpu)
+    ops.paged_prefill(q, kv[..., :64], kv[..., 64:], p.bt.to(gpu), p.cu.to(gpu), p.lens.to(gpu),
+                      0.125, max_seqlen_q=130, max_seqlen_k=2000, out=q)
+    out, _ = _run(p)
+    assert torch.equal(q, out)
+
+
+def test_two_streams_at_once(gpu):
+    """Divided calls on two streams, each with its own scratch and counters."""
+    ps = [po.Paged([60, 2], [2500, 3000], 8, 2, 64, torch.float16, seed=s) for s in (39, 40)]
+    dev = [dict(q=p.q.to(gpu), kv=p.kv.to(gpu), bt=p.bt.to(gpu), cu=p.cu.to(gpu), ln=p.lens.to(gpu))
+           for p in ps]
+    want = [_run(p) for p in ps]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for x, s, g in zip(dev, streams, got):
+            with torch.cuda.stream(s):
+                g.append(ops.paged_prefill(x["q"], x["kv"][..., :64], x["kv"][..., 64:], x["bt"],
+                                           x["cu"], x["ln"], 0.125, 60, 3000))
+    torch.cuda.synchronize()
+    for g, (out, lse) in zip(got, want):
+        for o, l in g:
+            assert torch.equal(o, out) and torch.equal(l, lse)
+
+
+@pytest.mark.parametrize("D", [128, 256, 72])
+def test_cache_offsets_past_32_bits(gpu, D):
+    """Blocks at the far end of a cache of more than 2^31 elements: the same bits as at its start."""
+    p = po.Paged([130, 2], [700, 400], 4, 2, D, torch.bfloat16, seed=44)
+    kv = p.kv.to(gpu)
+    elements = p.BS * 2 * 2 * D
+    far = 2 ** 31 // elements + 5
+    big = torch.empty(far + p.B, p.BS, 2, 2 * D, dtype=torch.bfloat16, device=gpu)
+    big[far:] = kv
+    want = _run(p)
+    bt = torch.where(p.bt >= 0, p.bt + far, p.bt)
+    got = _run(p, k=big[..., :D], v=big[..., D:], bt=bt)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    _check(p, *got)
