@@ -519,10 +519,9 @@ int fd_build_tables(
  * fd_paged_decode_counted (the same array may serve both, in stream order),
  * which save a call whose rows are divided among workgroups the launch that
  * clears counters in the workspace.
- * Fast kernels: fp16 / bf16 with head_size a multiple of 16 up to 128, or
- * 256, and fp32 with head_size a multiple of 16 up to 256, where pointers
- * are 16-byte aligned and strides multiples of 16 bytes; anything else takes
- * a slower generic kernel.
+ * Fast kernels: head_size a multiple of 16 from 32 to 128, or 256, where
+ * pointers are 16-byte aligned and strides multiples of 16 bytes; anything
+ * else takes a slower generic kernel.
  * ------------------------------------------------------------------------ */
 int fd_paged_prefill(
     const void* q, int64_t q_stride_tok, int64_t q_stride_head,

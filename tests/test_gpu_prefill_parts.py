@@ -57,6 +57,29 @@ def test_many_tokens_over_many_keys(gpu, dtype, D):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 80, 128])
+def test_rows_of_few_tokens_beside_many(gpu, dtype, D):
+    """The same tiles, and short rows' tiles of eight waves beside them."""
+    H, qs, ks = 64, [3, 2100, 1, 64], [900, 4200, 1, 4100]
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q = torch.randn(sum(qs), H, D, generator=g, device=gpu).to(dtype)
+    k = torch.randn(sum(ks), H, D, generator=g, device=gpu).to(dtype)
+    v = torch.randn(sum(ks), H, D, generator=g, device=gpu).to(dtype)
+    cu_q, cu_k = po.starts(qs), po.starts(ks)
+    scale = 1 / math.sqrt(D)
+    out, lse = ops.varlen_attention(q, k, v, cu_q.to(gpu), cu_k.to(gpu), scale, max_seqlen_q=2100,
+                                    max_seqlen_k=4200, causal=True)
+    for h in (0, 33, 63):
+        qc, kc, vc = (x[:, h:h + 1].cpu() for x in (q, k, v))
+        for i, tokens in ((0, (0, 1, 2)), (1, (0, 63, 2047, 2099)), (2, (0,)), (3, (0, 31, 32, 63))):
+            for j in tokens:
+                t, k0 = int(cu_q[i]) + j, int(cu_k[i])
+                see = slice(k0, k0 + ks[i] - qs[i] + j + 1)
+                ref = po.attend(qc[t:t + 1], kc[see], vc[see], scale, False, out.dtype)
+                po.check(out[t:t + 1, h:h + 1], lse[h:h + 1, t:t + 1], ref, f"row {i} token {j} head {h}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [48, 64, 128, 256])
 @pytest.mark.parametrize("qs,ks", [([300], [4100]), ([3], [4100]), ([100, 37, 5], [2900, 40, 1500])],
                          ids=str)
